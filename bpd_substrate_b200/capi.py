@@ -196,6 +196,12 @@ SIGNATURES = {
     "bpdq_hybrid_logits": (vp, [vp]),
     "bpdq_hybrid_picked": (vp, [vp]),
     "bpdq_hybrid_scratch_bytes": (sz, [vp]),
+    # serving many sequences
+    "bpd_paged_append_cuda": (i32, [vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, vp, vp]),
+    "bpd_paged_attention_cuda": (i32, [vp, vp, i32, vp, i32, i32, f32, f32, vp, vp]),
+    "bpdq_paged_attention_workspace_bytes": (sz, [vp, i32, vp]),
+    "bpd_paged_attention_ws_cuda": (i32, [vp, vp, i32, vp, i32, i32, f32, f32, vp, vp, sz, vp]),
+    "bpd_sample_cuda": (i32, [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "gpu_matmul_q4k": (None, [vp, vp, vp, i32, i32, i32]),
 }
 
@@ -305,6 +311,20 @@ class HybridConfig(C.Structure):
     """bpdq_hybrid_config."""
     _fields_ = ([(n, i32) for n in ("n_layers", "width", "width_pad", "vocab", "act_bf16", "streams")]
                 + [(n, f32) for n in ("eps", "embed_scale", "logit_cap")] + [("embed", vp), ("head", vp), ("final_norm", DynTanh)])
+
+
+TYPE_F32, TYPE_F16, TYPE_BF16 = range(3)
+
+
+class PagedKv(C.Structure):
+    """bpdq_paged_kv."""
+    _fields_ = ([(n, i32) for n in ("heads", "kv_heads", "dim", "act_type", "kv_type", "page", "n_pages", "batch", "max_pages")] + [("page_stride", sz)]
+                + [(n, vp) for n in ("k", "v", "page_table", "length", "seq_start")])
+
+
+class PagedGroups(C.Structure):
+    """bpdq_paged_groups."""
+    _fields_ = [("n", i32), ("start", vp), ("pages", vp)]
 
 
 class BpdqError(RuntimeError):

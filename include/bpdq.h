@@ -590,6 +590,56 @@ float* bpdq_hybrid_logits(void* plan);                /* device [n_want][vocab] 
 void* bpdq_hybrid_picked(void* plan);                 /* device int64 [n_want] */
 size_t bpdq_hybrid_scratch_bytes(void* plan);
 
+/* ---- serving many sequences at once: a KV cache in pages, attention over it, sampling ----
+ * Beside the caches above, whose rows belong to one sequence: a pool of pages that sequences are given one by one and may share.
+ * Types of activations and cache: fp32 on fp16 (the Llama's), fp16 on fp16, bf16 on bf16. */
+enum { BPDQ_TYPE_F32 = 0, BPDQ_TYPE_F16 = 1, BPDQ_TYPE_BF16 = 2 };
+/* Host memory holding device pointers.  Position p of sequence b is row p % page of page page_table[b][p / page]; a page of either pool
+ * is [kv_heads][page][dim], pages lie page_stride elements apart (0: kv_heads * page * dim).  length[b]: positions of sequence b ahead of
+ * the call.  Its new tokens are rows seq_start[b] .. seq_start[b + 1] - 1 of the call's (in the order of the sequences; some may bring none;
+ * rows behind the last sequence's are left as they are), or row b with seq_start NULL.
+ * page: 8, 16 .. 256; dim: a multiple of 8 up to 128; up to 2048 sequences; kv_heads divides heads; pools 16-byte aligned.
+ * Tables and lengths are read on the device when the call's work runs, so a recorded call follows them.  A sequence whose length is negative or
+ * would outgrow its row of the table, or whose bounds make no sense, is skipped (its rows are left as they are), a page outside 0 .. n_pages - 1 is
+ * neither written nor read (its positions take no part in attention); bpdq_last_status() then reports -4. */
+typedef struct {
+    int heads, kv_heads, dim, act_type, kv_type, page, n_pages, batch, max_pages;
+    size_t page_stride;
+    void *k, *v;
+    const int32_t *page_table, *length, *seq_start;
+} bpdq_paged_kv;
+/* The queries q, keys k and values v of n_tokens tokens (rows ld_* elements apart, heads side by side): queries and keys are turned by their
+ * positions, queries stored in q_out (which may be q; both NULL: no queries), keys and values in their pages.  Of a head's first rot_dims (even, up
+ * to dim; 0: none) dimensions pair i, dimensions (2 i, 2 i + 1) with neighbours and (i, i + rot_dims / 2) without, turns by position * rot_freq[i]:
+ * the Llama's pairing and the hybrid decoders'.  Two tokens must not have the same place. */
+int bpd_paged_append_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* q_out, int ld_q_out, const void* k, int ld_k, const void* v, int ld_v,
+                          int n_tokens, int rot_dims, int neighbours, const float* rot_freq, void* stream);
+/* Sequences that begin with the same pages: sequences start[g] .. start[g + 1] - 1 (start[n] <= batch, n <= batch) share the first pages[g] entries of their rows of
+ * page_table, all filled before the call (pages[g] * page <= length of each of them; what goes beyond that is not taken to be shared).  Those keys are then read once for all of the group's
+ * tokens; without it the result is the same up to the order of the sums. */
+typedef struct {
+    int n;
+    const int32_t *start, *pages;
+} bpdq_paged_groups;
+/* o[t][h] = sum_j softmax_j(s_j) v_j over the positions up to the token's own, s = scale q.k, with cap > 0 then cap tanh(s / cap).  The tokens' own keys and values are in the cache
+ * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q.  fp32 activations keep fp32 sums' accuracy (queries and weights enter the tensor
+ * cores as two fp16 numbers each).  groups NULL: none.  A sequence's sums are split over the GPU by a rule on all lengths of the call: its last bits may depend
+ * on what else is in the batch.  Scratch: see "scratch memory" above; its size does not depend on lengths. */
+int bpd_paged_attention_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* o, int ld_o, int n_tokens, float scale, float cap,
+                             const bpdq_paged_groups* groups, void* stream);
+size_t bpdq_paged_attention_workspace_bytes(const bpdq_paged_kv* kv, int n_tokens, const bpdq_paged_groups* groups);
+int bpd_paged_attention_ws_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* o, int ld_o, int n_tokens, float scale, float cap,
+                                const bpdq_paged_groups* groups, void* workspace, size_t workspace_bytes, void* stream);
+/* A token per row of logits [rows][ld] (ld >= vocab, vocab up to 262144) from given random numbers u[r] in [0, 1).  With weights w_i = exp((x_i - max) / temperature), sorted by x (the lowest
+ * index first among equals): the first top_k of them (0 or less: all), of these the fewest whose weights reach top_p of theirs (1 or more: all; one at least), of these
+ * the ones with w >= min_p (0: all); then the first index, in the vocabulary's order, at which the sum of the kept weights exceeds u times
+ * their total.  temperature 0 (or anything not above 0): the largest logit.  Settings are device arrays [rows]; NULL: temperature 1, no cut.  NaN and -inf logits
+ * are never chosen; +inf beats all others; a row that has nothing else gives token -1 and log probability -inf.  logprob (or NULL): ln(w / total) of the token among the
+ * kept.  Weights are held to 2^-45 of the largest (a token with less is never chosen) and added as whole numbers, so a token depends neither on the order of sums nor on
+ * what else is in the batch. */
+int bpd_sample_cuda(const void* logits, int logits_type, int ld, int rows, int vocab, const float* temperature, const int32_t* top_k, const float* top_p,
+                    const float* min_p, const float* u, long long* token, float* logprob, void* stream);
+
 /* ---- row-sharded products on several GPUs without a collective.
  * The reference's decode loop runs on one GPU; with the rows of every matrix sharded over ranks (one
  * process per GPU) each rank needs the other ranks' output slices.  Instead of an all-gather after the
