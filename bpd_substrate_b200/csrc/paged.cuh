@@ -33,6 +33,11 @@ static inline size_t paged_stride(const bpdq_paged_kv& kv) { return kv.page_stri
 
 #ifdef __CUDACC__
 
+__device__ __forceinline__ void report(int* err, int code)
+{
+    if (err) atomicCAS(err, 0, code);
+}
+
 // What a sequence brings to a call.  A sequence whose numbers make no sense (a negative length, more tokens than its row of the page table holds,
 // bounds that run backwards or beyond the call's tokens) brings nothing, and the error word says so.
 struct PagedSpan {
@@ -46,7 +51,7 @@ __device__ __forceinline__ PagedSpan paged_span(const int* __restrict__ seq_star
     s.held = length[b];
     if (s.count == 0) return s;
     if (s.first < 0 || s.count < 0 || s.count > n_tokens || s.first > n_tokens - s.count || s.held < 0 || s.held > capacity - s.count) {
-        atomicCAS(err, 0, 81);
+        report(err, 81);
         s.count = 0;
     }
     return s;

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArg
     if (tid == 0) {
         const int page = p.table[(size_t)s_seq * p.max_pages + pos / p.page];
         s_page = page >= 0 && page < p.n_pages ? page : -1;
-        if (s_page < 0) atomicCAS(err, 0, 82);
+        if (s_page < 0) report(err, 82);
     }
     if (tid < half) {
         // in half turns: a / pi, less the nearest even number

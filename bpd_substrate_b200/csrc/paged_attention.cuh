@@ -1,0 +1,223 @@
+// Attention over a paged cache: what its kernels share.  A call's work is cut into jobs, a set of rows (row = (token, query head of a key head)) against
+// a range of positions: every sequence's new tokens against its own positions, and every group's tokens against the pages that the group shares.  A
+// job has an item per key head.  Items are laid end to end in units of keys and dealt to the CTAs in equal portions, whatever the lengths; an item
+// that several CTAs have parts of, or that has a prefix, leaves its parts in scratch memory, and k_paged_join adds them up.
+#pragma once
+#include "paged.cuh"
+#include "tensor_map.cuh"
+
+namespace bpdq {
+
+struct PagedArgs {
+    const void *q, *k_pool, *v_pool;
+    void* o;
+    int ld_q, ld_o;
+    int n_tokens, batch, heads, kv_heads, share, dim, page, log_page, max_pages, n_pages;
+    size_t page_stride;
+    const int *seq_start, *length, *table;
+    int groups;
+    const int *group_start, *group_pages;
+    float scale, cap;
+    int split_rows;             // jobs of up to so many rows are k_paged_split's, the others k_paged_tile's
+    int mark;                   // this launch says which tokens belong to no sequence
+    // scratch
+    int4* own;                  // [tokens][heads]: what k_paged_join finds of a row's own positions
+    int4* prefix;               // the same of its group's
+    float *own_o, *prefix_o;    // [tokens * heads][dim_pad]: parts that are whole, unnormalised
+    float2 *own_ml, *prefix_ml; // their maxima (in units of log2) and sums
+    float *split_o, *tile_o;    // parts of items that several CTAs share: [2 * CTA + which][rows][dim_pad]
+    float2 *split_ml, *tile_ml;
+    float* head_o;              // k_paged_split: a warp's first part, when it has two
+    float2* head_ml;
+};
+
+// A row's descriptor: x the CTA with the first part, y the number of parts (0: the row belongs to no sequence; 1: all in one CTA), z the row within the
+// parts, w: flags
+constexpr int kJoinTile = 1;            // parts are k_paged_tile's
+constexpr int kJoinPrefix = 2;          // (own) the row has a prefix as well
+constexpr int kSplitRows = 16, kTileRows = 256;
+
+// 4-D tiles (64 dimensions, up to 16 positions of a page, a head, a page) of a pool in the 128-byte swizzle; dimensions beyond the head's read as zeros.
+static inline int paged_map(CUtensorMap* map, const void* pool, const bpdq_paged_kv& kv, int rows)
+{
+    const cuuint64_t dims[4] = {(cuuint64_t)kv.dim, (cuuint64_t)kv.page, (cuuint64_t)kv.kv_heads, (cuuint64_t)kv.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)kv.dim * 2, (cuuint64_t)kv.page * kv.dim * 2, (cuuint64_t)paged_stride(kv) * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(kv.page < rows ? kv.page : rows), 1, 1};
+    return swizzled_map(map, pool, 4, dims, strides, box);
+}
+
+// paged_split.cu, paged_tile.cu
+int paged_split(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s);
+constexpr int kSplitWarps = 8;
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, int d, int row, int head, int page, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(d), "r"(row), "r"(head), "r"(page), "r"(bar)
+        : "memory");
+}
+
+// cap tanh(x / cap): of fp32 results by CUDA's function, of rounded ones by 1 - 2 / (1 + e^(2 x / cap)), off by 2^-22 of the cap.
+template <bool kExact> __device__ __forceinline__ float capped(float x, float cap)
+{
+    if (kExact) return cap * tanhf(x / cap);
+    return cap - __fdividef(2.0f * cap, 1.0f + ex2(2.88539008177792681f * __fdividef(x, cap)));
+}
+
+// The jobs of a call, as every CTA works them out for itself.  cum[j]: units ahead of job j; jobs 0 .. batch - 1 are the sequences', the groups' follow.
+struct PagedJob {
+    int first, count, rows;         // tokens, rows
+    int from, to;                   // positions
+    int seq;                        // whose row of the page table
+    bool prefix, joined;            // a group's job; rows that k_paged_join meets in any case
+};
+struct PagedPlan {
+    int* cum;                       // shared, [jobs + 1]
+    int* group_len;                 // shared, [groups]: positions that a group shares
+    int jobs;
+
+    __device__ static int size(const PagedArgs& p) { return (p.batch + 2 * p.groups + 2) * 4; }
+    // The group of a sequence, or -1.
+    __device__ static int group_of(const PagedArgs& p, int b)
+    {
+        int lo = 0, hi = p.groups;                      // start[lo] <= b < start[hi]
+        if (!p.groups || b < p.group_start[0] || b >= p.group_start[p.groups]) return -1;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (p.group_start[mid] <= b) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+    __device__ static PagedSpan span(const PagedArgs& p, int b, int* err)
+    {
+        return paged_span(p.seq_start, p.length, b, p.n_tokens, p.max_pages * p.page, err);
+    }
+    __device__ static void members(const PagedArgs& p, int g, int& s0, int& s1)
+    {
+        s0 = min(max(p.group_start[g], 0), p.batch);
+        s1 = min(max(p.group_start[g + 1], s0), p.batch);
+    }
+    __device__ PagedJob job(const PagedArgs& p, int j, int* err) const
+    {
+        PagedJob r;
+        r.prefix = j >= p.batch;
+        if (!r.prefix) {
+            const PagedSpan s = span(p, j, err);
+            const int g = group_of(p, j);
+            r.first = s.first; r.count = s.count; r.seq = j;
+            r.from = g >= 0 ? group_len[g] : 0;
+            r.to = s.held + s.count;
+            r.joined = r.from > 0;
+        } else {
+            int s0, s1;
+            members(p, j - p.batch, s0, s1);
+            // a group's tokens lie side by side: its sequences do
+            const int a = p.seq_start ? p.seq_start[s0] : s0, b = p.seq_start ? p.seq_start[s1] : s1;
+            r.first = min(max(a, 0), p.n_tokens);
+            r.count = min(max(b, r.first), p.n_tokens) - r.first;
+            r.seq = min(s0, p.batch - 1);
+            r.from = 0;
+            r.to = group_len[j - p.batch];
+            r.joined = true;
+            if (r.to <= 0) r.count = 0;
+        }
+        r.rows = r.count * p.share;
+        return r;
+    }
+    // units(job): those of one of its items, 0 for a job that is not this kernel's.  All threads of the CTA; returns the units in all.
+    template <int kThreads, class Units>
+    __device__ int build(const PagedArgs& p, int* shared, int* err, Units units)
+    {
+        __shared__ int s_warp[kThreads / 32], s_total;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        jobs = p.batch + p.groups;
+        cum = shared;
+        group_len = shared + jobs + 1;
+        if (p.groups) {
+            for (int g = tid; g < p.groups; g += kThreads) group_len[g] = min(max(p.group_pages[g], 0), p.max_pages) * p.page;
+            __syncthreads();
+            for (int b = tid; b < p.batch; b += kThreads) {
+                const int g = group_of(p, b);
+                if (g < 0) continue;
+                const PagedSpan s = span(p, b, err);
+                if (s.count > 0) atomicMin(&group_len[g], s.held);
+            }
+            __syncthreads();
+            for (int g = tid; g < p.groups; g += kThreads) {
+                int s0, s1;
+                members(p, g, s0, s1);
+                group_len[g] = s1 - s0 > 1 ? group_len[g] / p.page * p.page : 0;
+            }
+            __syncthreads();
+        }
+        int run = 0;
+        for (int j0 = 0; j0 < jobs; j0 += kThreads) {
+            const int j = j0 + tid;
+            int n = 0;
+            if (j < jobs) {
+                const PagedJob r = job(p, j, err);
+                if (r.rows > 0 && r.to > r.from) n = units(r) * p.kv_heads;
+            }
+            int up = n;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, up, o);
+                if (lane >= o) up += v;
+            }
+            if (lane == 31) s_warp[warp] = up;
+            __syncthreads();
+            int before = run;
+            for (int w = 0; w < warp; w++) before += s_warp[w];
+            if (j < jobs) cum[j] = before + up - n;
+            if (tid == kThreads - 1) s_total = before + up;
+            __syncthreads();
+            run = s_total;
+        }
+        if (tid == 0) cum[jobs] = run;
+        __syncthreads();
+        return run;
+    }
+    // The job that unit u belongs to.
+    __device__ __forceinline__ int find(int u) const
+    {
+        int lo = 0, hi = jobs;                          // cum[lo] <= u < cum[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (cum[mid] <= u) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+
+// The launch's share of the tokens that belong to no sequence: k_paged_join passes them over.
+template <int kThreads>
+__device__ __forceinline__ void mark_tokens(const PagedArgs& p, int* err)
+{
+    for (int t = blockIdx.x * kThreads + threadIdx.x; t < p.n_tokens; t += gridDim.x * kThreads) {
+        int b = t;
+        if (p.seq_start) {
+            int lo = 0, hi = p.batch;                   // the last sequence that starts at or before t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (p.seq_start[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            b = lo;
+        }
+        bool mine = false;
+        if (b < p.batch) {
+            const PagedSpan s = PagedPlan::span(p, b, err);
+            mine = s.count > 0 && s.first <= t && t < s.first + s.count;
+        }
+        if (!mine)
+            for (int h = 0; h < p.heads; h++) p.own[(size_t)t * p.heads + h] = make_int4(0, 0, 0, 0);
+    }
+}
+
+#endif
+}  // namespace bpdq
