@@ -1,74 +1,9 @@
-// Attention of new tokens over a paged cache (paged.cuh).  A warp takes a (token, head) and walks the positions up to its own, 32 at a time: a lane scores a
-// position, and the running maximum and sum of the softmax are joined once per 32.
+// Attention of new tokens over a paged cache (paged_attention.cuh): which kernels a call takes, their scratch memory, and how parts are joined.
 #include "paged_attention.cuh"
 
 #include <type_traits>
 
 namespace bpdq {
-
-template <typename A, typename K>
-__global__ void __launch_bounds__(128) k_paged_attn_plain(const PagedArgs p, int* err)
-{
-    __shared__ float s_q[4][kPagedMaxDim];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int item = blockIdx.x * 4 + warp;
-    pdl_launch_dependents();
-    pdl_wait();
-    if (item >= p.n_tokens * p.heads) return;
-    const int t = item / p.heads, h = item % p.heads, g = h / (p.heads / p.kv_heads);
-    int seq = -1, pos = 0;
-    for (int b0 = 0; b0 < p.batch && seq < 0; b0 += 32) {
-        const int b = b0 + lane;
-        PagedSpan s = {0, 0, 0};
-        if (b < p.batch) s = paged_span(p.seq_start, p.length, b, p.n_tokens, p.max_pages * p.page, err);
-        const unsigned hit = __ballot_sync(0xFFFFFFFFu, s.count > 0 && s.first <= t && t < s.first + s.count);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            seq = b0 + src;
-            pos = __shfl_sync(0xFFFFFFFFu, s.held + t - s.first, src);
-        }
-    }
-    if (seq < 0) return;
-    const A* q = static_cast<const A*>(p.q) + (size_t)t * p.ld_q + h * p.dim;
-    for (int d = lane; d < p.dim; d += 32) s_q[warp][d] = ActOf<A>::get(q[d]);
-    __syncwarp();
-    float m = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j0 = 0; j0 <= pos; j0 += 32) {
-        const int j = j0 + lane;
-        float x = -INFINITY;
-        long at = -1;
-        if (j <= pos) {
-            const int page = p.table[(size_t)seq * p.max_pages + j / p.page];
-            if (page >= 0 && page < p.n_pages) {
-                at = (long)((size_t)page * p.page_stride + ((size_t)g * p.page + j % p.page) * p.dim);
-                const K* k = static_cast<const K*>(p.k_pool) + at;
-                float s = 0.0f;
-                for (int d = 0; d < p.dim; d++) s = fmaf(s_q[warp][d], ActOf<K>::get(k[d]), s);
-                x = s * p.scale;
-                if (p.cap > 0.0f) x = p.cap * tanhf(x / p.cap);
-            } else {
-                report(err, 82);
-            }
-        }
-        const float top = fmaxf(m, warp_max(x)), base = top == -INFINITY ? 0.0f : top;
-        const float down = expf(m - base), w = at < 0 ? 0.0f : expf(x - base);
-        sum = sum * down + warp_sum(w);
-        m = top;
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] *= down;
-        for (int l = 0; l < 32; l++) {
-            const float wl = __shfl_sync(0xFFFFFFFFu, w, l);
-            const long al = __shfl_sync(0xFFFFFFFFu, at, l);
-            if (al < 0) continue;
-            const K* v = static_cast<const K*>(p.v_pool) + al;
-            for (int i = 0; i < 4; i++)
-                if (32 * i + lane < p.dim) acc[i] = fmaf(wl, ActOf<K>::get(v[32 * i + lane]), acc[i]);
-        }
-    }
-    A* o = static_cast<A*>(p.o) + (size_t)t * p.ld_o + h * p.dim;
-    for (int i = 0; i < 4; i++)
-        if (32 * i + lane < p.dim) o[32 * i + lane] = ActOf<A>::put(sum > 0.0f ? acc[i] / sum : 0.0f);
-}
 
 static int check_groups(const bpdq_paged_kv* kv, const bpdq_paged_groups* g)
 {
@@ -225,7 +160,8 @@ static int attention_check(const bpdq_paged_kv* kv, int n_tokens, const bpdq_pag
 {
     int rc = paged_check(kv, n_tokens);
     if (rc || (rc = check_groups(kv, groups))) return rc;
-    // units of work are counted in 32 bits
+    // a tile of rows holds a token's at least; units of work are counted in 32 bits
+    if (kv->heads / kv->kv_heads > 128) return latch(BPDQ_ERR_RANGE);
     return (double)kv->batch * kv->kv_heads * kv->max_pages * kv->page > 8589934592.0 ? latch(BPDQ_ERR_RANGE) : 0;
 }
 
@@ -240,6 +176,20 @@ static PagedArgs arguments(const bpdq_paged_kv& kv, int n_tokens, const bpdq_pag
     return p;
 }
 
+// Which kernels a call needs.  The host does not know lengths or bounds: where a job may have more rows than k_paged_split takes, both are launched, and each passes over the
+// other's jobs.
+struct Kernels {
+    int split_rows;         // jobs of up to so many rows go to k_paged_split; 0: it is not launched
+    bool tile;
+};
+static Kernels kernels(const PagedArgs& p)
+{
+    Kernels k;
+    k.split_rows = p.share > kSplitRows ? 0 : (p.share <= 8 && !p.seq_start ? 8 : kSplitRows);
+    k.tile = p.seq_start || p.groups || !k.split_rows;
+    return k;
+}
+
 static int paged_attention(const bpdq_paged_kv* kv, const void* q, int ld_q, void* o, int ld_o, int n_tokens, float scale, float cap, const bpdq_paged_groups* groups,
                            Workspace* ws, cudaStream_t s)
 {
@@ -251,24 +201,25 @@ static int paged_attention(const bpdq_paged_kv* kv, const void* q, int ld_q, voi
     if ((((uintptr_t)q | (uintptr_t)o) & 15) || ld_q % unit || ld_o % unit) return latch(BPDQ_ERR_ALIGN);
     if (n_tokens == 0 || kv->batch == 0) return 0;
     PagedArgs p = arguments(*kv, n_tokens, groups);
-    p.k_pool = kv->k; p.v_pool = kv->v; p.q = q; p.o = o; p.ld_q = ld_q; p.ld_o = ld_o; p.scale = scale; p.cap = cap;
+    p.q = q; p.o = o; p.ld_q = ld_q; p.ld_o = ld_o; p.scale = scale; p.cap = cap;
     const int ctas = sm_count();
-    if (!kv->seq_start && p.share <= kSplitRows && !p.groups) {
-        uint8_t* mem = scratch_take(ws, kScratchPaged, carve(p, nullptr, ctas, false), s, &rc);
-        if (!mem) return rc;
-        carve(p, mem, ctas, false);
-        p.split_rows = p.share;
+    const Kernels run = kernels(p);
+    uint8_t* mem = scratch_take(ws, kScratchPaged, carve(p, nullptr, ctas, run.tile), s, &rc);
+    if (!mem) return rc;
+    carve(p, mem, ctas, run.tile);
+    p.split_rows = run.split_rows;
+    if (run.tile) {
+        p.mark = !run.split_rows;
+        if ((rc = paged_tile(p, *kv, ctas, s))) return rc;
+    }
+    if (run.split_rows) {
         p.mark = 1;
         if ((rc = paged_split(p, *kv, ctas, s))) return rc;
-        const bool wide = kv->dim > 64;
-        if (kv->act_type == BPDQ_TYPE_F32) return wide ? launch_join<float, 128>(p, s) : launch_join<float, 64>(p, s);
-        if (kv->act_type == BPDQ_TYPE_F16) return wide ? launch_join<__half, 128>(p, s) : launch_join<__half, 64>(p, s);
-        return wide ? launch_join<bf16, 128>(p, s) : launch_join<bf16, 64>(p, s);
     }
-    const dim3 grid((unsigned)((n_tokens * kv->heads + 3) / 4));
-    if (kv->act_type == BPDQ_TYPE_F32) return launch_ordered(k_paged_attn_plain<float, __half>, grid, 128, 0, s, p, device_error_flag());
-    if (kv->act_type == BPDQ_TYPE_F16) return launch_ordered(k_paged_attn_plain<__half, __half>, grid, 128, 0, s, p, device_error_flag());
-    return launch_ordered(k_paged_attn_plain<bf16, bf16>, grid, 128, 0, s, p, device_error_flag());
+    const bool wide = kv->dim > 64;
+    if (kv->act_type == BPDQ_TYPE_F32) return wide ? launch_join<float, 128>(p, s) : launch_join<float, 64>(p, s);
+    if (kv->act_type == BPDQ_TYPE_F16) return wide ? launch_join<__half, 128>(p, s) : launch_join<__half, 64>(p, s);
+    return wide ? launch_join<bf16, 128>(p, s) : launch_join<bf16, 64>(p, s);
 }
 
 }  // namespace bpdq
@@ -287,7 +238,7 @@ size_t bpdq_paged_attention_workspace_bytes(const bpdq_paged_kv* kv, int n_token
 {
     if (attention_check(kv, n_tokens, groups)) return 0;
     PagedArgs p = arguments(*kv, n_tokens, groups);
-    return carve(p, nullptr, sm_count(), false) + 256;
+    return carve(p, nullptr, sm_count(), kernels(p).tile) + 256;
 }
 
 int bpd_paged_attention_ws_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* o, int ld_o, int n_tokens, float scale, float cap,

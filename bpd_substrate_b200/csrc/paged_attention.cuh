@@ -9,7 +9,7 @@
 namespace bpdq {
 
 struct PagedArgs {
-    const void *q, *k_pool, *v_pool;
+    const void* q;
     void* o;
     int ld_q, ld_o;
     int n_tokens, batch, heads, kv_heads, share, dim, page, log_page, max_pages, n_pages;
@@ -48,6 +48,7 @@ static inline int paged_map(CUtensorMap* map, const void* pool, const bpdq_paged
 
 // paged_split.cu, paged_tile.cu
 int paged_split(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s);
+int paged_tile(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s);
 constexpr int kSplitWarps = 8;
 
 #ifdef __CUDACC__

@@ -77,6 +77,14 @@ def test_bad_groups(lib, n, start, pages):
     lib.bpdq_clear_status()
 
 
+@pytest.mark.parametrize("changes", [dict(heads=258, kv_heads=2), dict(batch=2048, max_pages=1 << 21)])
+def test_attention_beyond_its_range(lib, changes):
+    kv = paged(**changes)
+    assert attention(lib, kv, ld_q=258 * 64, ld_o=258 * 64) == -3
+    assert lib.bpdq_paged_attention_workspace_bytes(C.byref(kv), 5, None) == 0
+    lib.bpdq_clear_status()
+
+
 def test_no_descriptor_and_no_workspace(lib):
     assert append(lib, None) == -1 and attention(lib, None) == -1
     assert lib.bpdq_paged_attention_workspace_bytes(None, 5, None) == 0
