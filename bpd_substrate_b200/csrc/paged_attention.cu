@@ -57,13 +57,14 @@ __global__ void __launch_bounds__(128) k_paged_join(const PagedArgs p)
             float most = -INFINITY, l = 0.0f, acc[kCols];
 #pragma unroll
             for (int c = 0; c < kCols; c++) acc[c] = 0.0f;
-            for (int i0 = 32 * member; i0 < n; i0 += 32 * TEAM) {
-                // maxima and sums of up to 32 parts, a lane each
-                const float *o = nullptr;
+            // the member's parts: member, member + TEAM, ..; their maxima and sums a lane each, their outputs eight at a time
+            for (int i0 = 0; i0 * TEAM + member < n; i0 += 32) {
+                const int i = (i0 + lane) * TEAM + member;
+                const float* o = p.own_o;
                 const float2* ml = nullptr;
                 float2 v = make_float2(-INFINITY, 0.0f);
-                if (i0 + lane < n) {
-                    place(i0 + lane, o, ml);
+                if (i < n) {
+                    place(i, o, ml);
                     v = *ml;
                 }
                 const float top = fmaxf(most, warp_max(v.x)), ref = top == -INFINITY ? 0.0f : top, down = ex2(most - ref);
@@ -72,21 +73,24 @@ __global__ void __launch_bounds__(128) k_paged_join(const PagedArgs p)
                 most = top;
 #pragma unroll
                 for (int c = 0; c < kCols; c++) acc[c] *= down;
-                const int here = n - i0 < 32 ? n - i0 : 32;
-#pragma unroll 4
-                for (int i = 0; i < here; i++) {
-                    const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
-                    const float* from = reinterpret_cast<const float*>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)o, i)) + kCols * lane;
-                    if (kCols == 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(from);
-                        acc[0] = fmaf(wi, x.x, acc[0]);
-                        acc[1] = fmaf(wi, x.y, acc[1]);
-                        acc[kCols - 2] = fmaf(wi, x.z, acc[kCols - 2]);
-                        acc[kCols - 1] = fmaf(wi, x.w, acc[kCols - 1]);
-                    } else {
-                        const float2 x = *reinterpret_cast<const float2*>(from);
-                        acc[0] = fmaf(wi, x.x, acc[0]);
-                        acc[1] = fmaf(wi, x.y, acc[1]);
+                const int here = min(32, (n - member + TEAM - 1) / TEAM - i0);
+                for (int k0 = 0; k0 < here; k0 += 8) {
+                    float x[8][kCols];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float* from = reinterpret_cast<const float*>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)o, k0 + k)) + kCols * lane;
+#pragma unroll
+                        for (int c = 0; c < kCols; c++) x[k][c] = 0.0f;
+                        if (k0 + k < here) {
+                            if constexpr (kCols == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(from);
+                            else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float wk = __shfl_sync(0xFFFFFFFFu, w, k0 + k);
+#pragma unroll
+                        for (int c = 0; c < kCols; c++) acc[c] = fmaf(wk, x[k][c], acc[c]);
                     }
                 }
             }
@@ -161,7 +165,7 @@ static int attention_check(const bpdq_paged_kv* kv, int n_tokens, const bpdq_pag
     int rc = paged_check(kv, n_tokens);
     if (rc || (rc = check_groups(kv, groups))) return rc;
     // a tile of rows holds a token's at least; units of work are counted in 32 bits
-    if (kv->heads / kv->kv_heads > 128) return latch(BPDQ_ERR_RANGE);
+    if (kv->heads / kv->kv_heads > 128 || kv->batch + (groups ? groups->n : 0) > kPagedMaxJobs) return latch(BPDQ_ERR_RANGE);
     return (double)kv->batch * kv->kv_heads * kv->max_pages * kv->page > 8589934592.0 ? latch(BPDQ_ERR_RANGE) : 0;
 }
 

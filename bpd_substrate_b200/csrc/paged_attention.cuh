@@ -19,6 +19,7 @@ struct PagedArgs {
     const int *group_start, *group_pages;
     float scale, cap;
     int split_rows;             // jobs of up to so many rows are k_paged_split's, the others k_paged_tile's
+    int both;                   // this launch's requests bring both halves of 128 dimensions
     int mark;                   // this launch says which tokens belong to no sequence
     // scratch
     int4* own;                  // [tokens][heads]: what k_paged_join finds of a row's own positions
@@ -36,14 +37,19 @@ struct PagedArgs {
 constexpr int kJoinTile = 1;            // parts are k_paged_tile's
 constexpr int kJoinPrefix = 2;          // (own) the row has a prefix as well
 constexpr int kSplitRows = 16, kTileRows = 256;
+constexpr int kPagedMaxJobs = 1280;      // sequences and groups of a call: 20 to 24 bytes of shared memory each
 
-// 4-D tiles (64 dimensions, up to 16 positions of a page, a head, a page) of a pool in the 128-byte swizzle; dimensions beyond the head's read as zeros.
+// Tiles of a pool in the 128-byte swizzle: up to `rows` positions of a head of a page, 64 dimensions wide, or (paged_both) both halves of 128 dimensions,
+// one behind the other, in one request.  Dimensions beyond the head's read as zeros.
+static inline bool paged_both(const bpdq_paged_kv& kv, int rows) { return kv.dim == 128 && kv.page >= rows; }
 static inline int paged_map(CUtensorMap* map, const void* pool, const bpdq_paged_kv& kv, int rows)
 {
-    const cuuint64_t dims[4] = {(cuuint64_t)kv.dim, (cuuint64_t)kv.page, (cuuint64_t)kv.kv_heads, (cuuint64_t)kv.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)kv.dim * 2, (cuuint64_t)kv.page * kv.dim * 2, (cuuint64_t)paged_stride(kv) * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(kv.page < rows ? kv.page : rows), 1, 1};
-    return swizzled_map(map, pool, 4, dims, strides, box);
+    const bool both = paged_both(kv, rows);
+    const cuuint64_t row = (cuuint64_t)kv.dim * 2;
+    const cuuint64_t dims[5] = {(cuuint64_t)(both ? 64 : kv.dim), (cuuint64_t)kv.page, (cuuint64_t)(both ? 2 : 1), (cuuint64_t)kv.kv_heads, (cuuint64_t)kv.n_pages};
+    const cuuint64_t strides[4] = {row, both ? 128 : row, row * kv.page, (cuuint64_t)paged_stride(kv) * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)(kv.page < rows ? kv.page : rows), (cuuint32_t)(both ? 2 : 1), 1, 1};
+    return swizzled_map(map, pool, 5, dims, strides, box);
 }
 
 // paged_split.cu, paged_tile.cu
@@ -53,11 +59,12 @@ constexpr int kSplitWarps = 8;
 
 #ifdef __CUDACC__
 
+// Rows of a page from dimension d (a multiple of 64) on; where both halves come in one request d is 0.
 __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, int d, int row, int head, int page, uint32_t bar)
 {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(map), "r"(d), "r"(row), "r"(head), "r"(page), "r"(bar)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(d), "r"(row), "r"(0), "r"(head), "r"(page), "r"(bar)
         : "memory");
 }
 
@@ -78,9 +85,10 @@ struct PagedJob {
 struct PagedPlan {
     int* cum;                       // shared, [jobs + 1]
     int* group_len;                 // shared, [groups]: positions that a group shares
+    int4* spans;                    // shared, [jobs]: first token, number of tokens, positions from, to
     int jobs;
 
-    __device__ static int size(const PagedArgs& p) { return (p.batch + 2 * p.groups + 2) * 4; }
+    __host__ __device__ static int size(const PagedArgs& p) { return 16 * (p.batch + p.groups) + 4 * (p.batch + 2 * p.groups + 1); }
     // The group of a sequence, or -1.
     __device__ static int group_of(const PagedArgs& p, int b)
     {
@@ -129,6 +137,29 @@ struct PagedPlan {
         r.rows = r.count * p.share;
         return r;
     }
+    __device__ __forceinline__ void keep(const PagedArgs& p, int j, const PagedJob& r)
+    {
+        if (p.mark && blockIdx.x == 0 && !p.seq_start && !r.prefix && r.count == 0)
+            for (int h = 0; h < p.heads; h++) p.own[(size_t)j * p.heads + h] = make_int4(0, 0, 0, 0);
+        spans[j] = make_int4(r.first, r.count, r.from, r.to);
+    }
+    // Job j, once the plan is built.
+    __device__ __forceinline__ PagedJob known(const PagedArgs& p, int j) const
+    {
+        const int4 s = spans[j];
+        PagedJob r;
+        r.prefix = j >= p.batch;
+        r.first = s.x; r.count = s.y; r.from = s.z; r.to = s.w;
+        r.rows = r.count * p.share;
+        r.joined = r.prefix || r.from > 0;
+        r.seq = j;
+        if (r.prefix) {
+            int s0, s1;
+            members(p, j - p.batch, s0, s1);
+            r.seq = min(s0, p.batch - 1);
+        }
+        return r;
+    }
     // units(job): those of one of its items, 0 for a job that is not this kernel's.  All threads of the CTA; returns the units in all.
     template <int kThreads, class Units>
     __device__ int build(const PagedArgs& p, int* shared, int* err, Units units)
@@ -136,8 +167,9 @@ struct PagedPlan {
         __shared__ int s_warp[kThreads / 32], s_total;
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
         jobs = p.batch + p.groups;
-        cum = shared;
-        group_len = shared + jobs + 1;
+        spans = reinterpret_cast<int4*>(shared);
+        cum = shared + 4 * jobs;
+        group_len = cum + jobs + 1;
         if (p.groups) {
             for (int g = tid; g < p.groups; g += kThreads) group_len[g] = min(max(p.group_pages[g], 0), p.max_pages) * p.page;
             __syncthreads();
@@ -156,11 +188,13 @@ struct PagedPlan {
             __syncthreads();
         }
         int run = 0;
+#pragma unroll 1
         for (int j0 = 0; j0 < jobs; j0 += kThreads) {
             const int j = j0 + tid;
             int n = 0;
             if (j < jobs) {
                 const PagedJob r = job(p, j, err);
+                keep(p, j, r);
                 if (r.rows > 0 && r.to > r.from) n = units(r) * p.kv_heads;
             }
             int up = n;
@@ -195,12 +229,20 @@ struct PagedPlan {
     }
 };
 
-// The launch's share of the tokens that belong to no sequence: k_paged_join passes them over.
-template <int kThreads>
-__device__ __forceinline__ void mark_tokens(const PagedArgs& p, int* err)
+// Units dealt to CTAs in equal runs, the first ones a unit longer where they do not come out even.
+struct PagedDeal {
+    int each, longer;               // units of a run; how many runs have one more
+    __device__ __forceinline__ PagedDeal(int total, int ctas) : each(total / ctas), longer(total - total / ctas * ctas) {}
+    __device__ __forceinline__ int first(int cta) const { return cta * each + min(cta, longer); }
+    __device__ __forceinline__ int cta_of(int u) const { return u < longer * (each + 1) ? u / (each + 1) : longer + (u - longer * (each + 1)) / each; }
+};
+
+// The tokens that belong to no sequence, strided over `lanes` threads of every CTA: k_paged_join passes them over.  (Where every sequence brings one token, PagedPlan::build has
+// seen to sequences that are skipped.)
+__device__ __forceinline__ void mark_tokens(const PagedArgs& p, int lane, int lanes, int* err)
 {
-    for (int t = blockIdx.x * kThreads + threadIdx.x; t < p.n_tokens; t += gridDim.x * kThreads) {
-        int b = t;
+    for (int t = (p.seq_start ? 0 : p.batch) + blockIdx.x * lanes + lane; t < p.n_tokens; t += gridDim.x * lanes) {
+        bool mine = false;
         if (p.seq_start) {
             int lo = 0, hi = p.batch;                   // the last sequence that starts at or before t
             while (hi - lo > 1) {
@@ -208,11 +250,7 @@ __device__ __forceinline__ void mark_tokens(const PagedArgs& p, int* err)
                 if (p.seq_start[mid] <= t) lo = mid;
                 else hi = mid;
             }
-            b = lo;
-        }
-        bool mine = false;
-        if (b < p.batch) {
-            const PagedSpan s = PagedPlan::span(p, b, err);
+            const PagedSpan s = PagedPlan::span(p, lo, err);
             mine = s.count > 0 && s.first <= t && t < s.first + s.count;
         }
         if (!mine)

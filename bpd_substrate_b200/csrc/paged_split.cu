@@ -11,15 +11,21 @@
 namespace bpdq {
 
 constexpr int kPsWarps = kSplitWarps, kPsThreads = 32 * kPsWarps, kPsKeys = 16, kPsRing = 24576;        // bytes of a warp's ring
+constexpr int kPsItems = 8;                         // more than copies can be ahead (six tiles)
 constexpr float kPsGrowth = 8.0f;                   // log2 of how far weights may exceed 1 before outputs are rescaled
 
 template <typename K> __device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void mma_16<bf16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_bf16(d, a, b0, b1); }
+template <> __device__ __forceinline__ void mma_16<bf16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 template <> __device__ __forceinline__ void mma_16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <typename K> __device__ __forceinline__ void split_16(float v0, float v1, uint32_t& hi, uint32_t& lo);
 template <> __device__ __forceinline__ void split_16<bf16>(float v0, float v1, uint32_t& hi, uint32_t& lo) { split_bf16(v0, v1, hi, lo); }
@@ -57,7 +63,7 @@ template <> __device__ __forceinline__ void store_two<bf16>(bf16* p, float a, fl
 // An item, and the unit of it that is next.
 struct PsItem {
     PagedJob job;
-    int j, head, begin, end, key;       // job, key head, its units, position of the next unit's first key
+    int tiles, head, begin, end, key;   // units of an item of the job, key head, its units, position of the next unit's first key
 };
 // What a warp leaves of an item that it has not all of.
 struct PsPart {
@@ -73,6 +79,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t bars[kPsWarps][kStages];
     __shared__ PsPart parts[kPsWarps][2];
+    __shared__ PsItem items[kPsWarps][kPsItems];        // as copies meet them, for the sums behind
     const uint32_t ring_all = (smem_addr(raw) + 1023) & ~1023u;
     uint8_t* ring_ptr = raw + (ring_all - smem_addr(raw));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -82,6 +89,16 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         mbar_init_fence();
     }
     if (lane < 2) parts[warp][lane].valid = 0;
+    if (tid == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    }
+    int row_tok[MT], row_head[MT];      // of the thread's rows: token within the job, query head within the key head's
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        row_tok[m] = (8 * m + g) / p.share;
+        row_head[m] = 8 * m + g - row_tok[m] * p.share;
+    }
     pdl_wait();
     pdl_launch_dependents();
 
@@ -90,33 +107,37 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                                              [&](const PagedJob& r) { return r.rows <= p.split_rows ? (r.to - r.from + kPsKeys - 1) / kPsKeys : 0; });
     // A tile per warp at least: fewer CTAs have fewer parts to join.
     const int most = (total + kPsWarps - 1) / kPsWarps, ctas = max(1, min((int)gridDim.x, most)), cta = blockIdx.x;
-    const int u0 = cta < ctas ? (int)((long long)total * cta / ctas) : total, u1 = cta < ctas ? (int)((long long)total * (cta + 1) / ctas) : total;
+    const PagedDeal deal(total, ctas);
+    const int u0 = cta < ctas ? deal.first(cta) : total, u1 = cta < ctas ? deal.first(cta + 1) : total;
     const int a0 = u0 + (u1 - u0) * warp / kPsWarps, a1 = u0 + (u1 - u0) * (warp + 1) / kPsWarps;
 
-    auto open = [&](PsItem& it, int u, bool again) {
-        if (!again || u >= plan.cum[it.j + 1]) {
-            it.j = plan.find(u);
-            it.job = plan.job(p, it.j, err);
-        }
-        const int tiles = (it.job.to - it.job.from + kPsKeys - 1) / kPsKeys, at = u - plan.cum[it.j];
-        it.head = at / tiles;
-        it.begin = plan.cum[it.j] + it.head * tiles;
-        it.end = it.begin + tiles;
-        it.key = it.job.from + (u - it.begin) * kPsKeys;
-    };
-
-    // ---- copies: the warp's tiles in order, kStages ahead
+    // ---- copies: the warp's tiles in order, kStages ahead.  (Code that runs once waits for its instructions: what follows is laid out so that nothing stands
+    // in it twice.)
     PsItem src = {};
-    int src_u = a0, entry = 0, entry_base = -1;
+    src.end = a0;
+    int src_u = a0, entry = 0, entry_base = 0, opened = 0;
     uint32_t missing = 0;               // two bits per stage: its first eight, its last eight positions have no page
     const bool small = p.page == 8;
     auto request = [&](int stage) {
-        if (src_u == a0 || src_u >= src.end) {
-            open(src, src_u, src_u != a0);
-            entry_base = -1;
+        if (src_u == src.end) {
+            if (opened && src.head + 1 < p.kv_heads) {
+                src.head++;
+                src.begin = src.end;
+            } else {
+                const int j = plan.find(src_u), at = src_u - plan.cum[j];
+                src.job = plan.known(p, j);
+                src.tiles = (src.job.to - src.job.from + kPsKeys - 1) / kPsKeys;
+                src.head = at / src.tiles;
+                src.begin = plan.cum[j] + src.head * src.tiles;
+            }
+            src.end = src.begin + src.tiles;
+            src.key = src.job.from + (src_u - src.begin) * kPsKeys;
+            if (lane == 0) items[warp][opened % kPsItems] = src;
+            opened++;
+            entry_base = -32;
         }
         const int e = src.key >> p.log_page;
-        if (entry_base < 0 || e + 1 >= entry_base + 32) {
+        if (e + 1 >= entry_base + 32) {
             entry_base = e;
             entry = e + lane < p.max_pages ? p.table[(size_t)src.job.seq * p.max_pages + e + lane] : -1;
         }
@@ -127,8 +148,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const uint32_t box = (uint32_t)((small ? 8 : kPsKeys) * 128 * kHalves * 2), n = small ? (ok0 ? 1u : 0u) + (ok1 ? 1u : 0u) : (ok0 ? 1u : 0u);
             mbar_expect_tx_at(bar, n * box);
             const int row = src.key & (p.page - 1);
-#pragma unroll
-            for (int h = 0; h < kHalves; h++) {
+            for (int h = 0; h < (p.both ? 1 : kHalves); h++) {
                 if (ok0) {
                     tma_page(at + h * (kPsKeys * 128), &kmap, 64 * h, row, src.head, page0, bar);
                     tma_page(at + kTile + h * (kPsKeys * 128), &vmap, 64 * h, row, src.head, page0, bar);
@@ -144,67 +164,73 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         src_u++;
         src.key += kPsKeys;
     };
-    for (int i = 0; i < kStages; i++)
-        if (src_u < a1) request(i);
-
-    // ---- sums
     PsItem it = {};
     uint32_t qf[MT][kSteps][f32 ? 4 : 2];           // queries: rows' (and their small parts') fragments
-    float out[MT][kOut][4], top[MT], sum[MT], factor[MT];
+    float factor[MT];
     int limit[MT];
-    bool alive = true;
-    int began = a0;                     // the unit with which the warp's part of the item began
-    for (int u = a0, n = 0; u < a1 && alive; u++, n++) {
-        const int stage = n % kStages;
-        if (u == a0 || u >= it.end) {
-            open(it, u, u != a0);
+    auto queries = [&] {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const bool live = 8 * m + g < it.job.rows;
+            const int tok = it.job.first + (live ? row_tok[m] : 0), h = it.head * p.share + (live ? row_head[m] : 0);
+            limit[m] = it.job.prefix ? it.job.to : it.job.to - it.job.count + (live ? row_tok[m] : 0) + 1;
+            const A* q = static_cast<const A*>(p.q) + (size_t)tok * p.ld_q + h * p.dim;
+            factor[m] = p.scale;
+            if constexpr (f32) {
+                float2 x[kSteps][2];
+                float big = 0.0f;
+#pragma unroll
+                for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int d = 16 * s + 8 * c + 2 * t4;
+                        x[s][c] = live && d < p.dim ? *reinterpret_cast<const float2*>(q + d) : make_float2(0.0f, 0.0f);
+                        big = fmaxf(big, fmaxf(fabsf(x[s][c].x), fabsf(x[s][c].y)));
+                    }
+                // a power of two brings the row's largest entry to 1 .. 2: both parts are then fp16 numbers, off by 2^-22 of it
+                big = quad_max(big);
+                const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big), -100), 100) : 0;
+                const float down = __int_as_float((127 - e) << 23);
+                factor[m] *= __int_as_float((127 + e) << 23);
+#pragma unroll
+                for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) split_16<K>(x[s][c].x * down, x[s][c].y * down, qf[m][s][2 * c], qf[m][s][2 * c + 1]);
+            } else {
+#pragma unroll
+                for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int d = 16 * s + 8 * c + 2 * t4;
+                        qf[m][s][c] = live && d < p.dim ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+                    }
+            }
+        }
+    };
+
+    // ---- sums
+    float out[MT][kOut][4], top[MT], sum[MT];
+    int began = a0, taken = 0;          // the unit with which the warp's part of the item began; items so far
+    // tile n is used, then the copy of tile n + kStages requested into its place
+#pragma unroll 1
+    for (int u = a0 - kStages, stage = 0, phase = 0; u < a1; u++) {
+      if (u >= a0) {
+        if (u == a0 || u == it.end) {
+            __syncwarp();
+            it = items[warp][taken++ % kPsItems];
+            queries();
             began = u;
 #pragma unroll
             for (int m = 0; m < MT; m++) {
-                const int r = 8 * m + g;
-                const bool live = r < it.job.rows;
-                const int tok = it.job.first + (live ? r / p.share : 0), h = it.head * p.share + (live ? r % p.share : 0);
-                limit[m] = it.job.prefix ? it.job.to : it.job.to - it.job.count + (live ? r / p.share : 0) + 1;
-                const A* q = static_cast<const A*>(p.q) + (size_t)tok * p.ld_q + h * p.dim;
                 top[m] = -INFINITY;
                 sum[m] = 0.0f;
-                factor[m] = p.scale;
-                if constexpr (f32) {
-                    float2 x[kSteps][2];
-                    float big = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < kSteps; s++)
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const int d = 16 * s + 8 * c + 2 * t4;
-                            x[s][c] = live && d < p.dim ? *reinterpret_cast<const float2*>(q + d) : make_float2(0.0f, 0.0f);
-                            big = fmaxf(big, fmaxf(fabsf(x[s][c].x), fabsf(x[s][c].y)));
-                        }
-                    // a power of two brings the row's largest entry to 1 .. 2: both parts are then fp16 numbers, off by 2^-22 of it
-                    big = quad_max(big);
-                    const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big), -100), 100) : 0;
-                    const float down = __int_as_float((127 - e) << 23);
-                    factor[m] *= __int_as_float((127 + e) << 23);
-#pragma unroll
-                    for (int s = 0; s < kSteps; s++)
-#pragma unroll
-                        for (int c = 0; c < 2; c++) split_16<K>(x[s][c].x * down, x[s][c].y * down, qf[m][s][2 * c], qf[m][s][2 * c + 1]);
-                } else {
-#pragma unroll
-                    for (int s = 0; s < kSteps; s++)
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const int d = 16 * s + 8 * c + 2 * t4;
-                            qf[m][s][c] = live && d < p.dim ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
-                        }
-                }
 #pragma unroll
                 for (int i = 0; i < kOut; i++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) out[m][i][c] = 0.0f;
             }
         }
-        if (!mbar_wait_bounded(&bars[warp][stage], (uint32_t)(n / kStages) & 1u, err, 83)) { alive = false; break; }
+        if (!mbar_wait_bounded(&bars[warp][stage], (uint32_t)phase, err, 83)) break;
         const uint32_t kt = ring + stage * 2 * kTile, vt = kt + kTile;
         const int have = min(kPsKeys, it.job.to - it.key);
         const uint32_t gone = missing >> (2 * stage) & 3u, valid = ((1u << have) - 1u) & ~((gone & 1u ? 0xFFu : 0u) | (gone & 2u ? 0xFF00u : 0u));
@@ -218,25 +244,30 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         }
-        float sc[MT][2][4];
+        // two chains of products per eight keys, fragments of four steps at a time
+        float sc[MT][2][4], sc2[MT][2][4];
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) sc[m][i >> 2][i & 3] = 0.0f;
+            for (int i = 0; i < 8; i++) sc[m][i >> 2][i & 3] = sc2[m][i >> 2][i & 3] = 0.0f;
         {
             const int r = (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
 #pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                uint32_t b[4];
-                ldsm4_at(b, kt + (s >> 2) * (kPsKeys * 128) + r * 128 + (((2 * (s & 3) + c) ^ (r & 7)) << 4));
+            for (int s0 = 0; s0 < kSteps; s0 += 4) {
+                uint32_t b[4][4];
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    uint32_t a[4];
-                    if constexpr (f32) { a[0] = qf[m][s][0]; a[1] = qf[m][s][1]; a[2] = qf[m][s][2]; a[3] = qf[m][s][3]; }
-                    else { a[0] = qf[m][s][0]; a[1] = 0; a[2] = qf[m][s][1]; a[3] = 0; }
-                    mma_16<K>(sc[m][0], a, b[0], b[1]);
-                    mma_16<K>(sc[m][1], a, b[2], b[3]);
-                }
+                for (int s = 0; s < 4; s++) ldsm4_at(b[s], kt + (s0 >> 2) * (kPsKeys * 128) + r * 128 + (((2 * s + c) ^ (r & 7)) << 4));
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        uint32_t a[4];
+                        const int q = s0 + s;
+                        if constexpr (f32) { a[0] = qf[m][q][0]; a[1] = qf[m][q][1]; a[2] = qf[m][q][2]; a[3] = qf[m][q][3]; }
+                        else { a[0] = qf[m][q][0]; a[1] = 0; a[2] = qf[m][q][1]; a[3] = 0; }
+                        mma_16<K>(s & 1 ? sc2[m][0] : sc[m][0], a, b[s][0], b[s][1]);
+                        mma_16<K>(s & 1 ? sc2[m][1] : sc[m][1], a, b[s][2], b[s][3]);
+                    }
             }
         }
         uint32_t w[MT][4];
@@ -248,8 +279,8 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                x[i] = sc[m][i >> 1][i & 1];
-                if constexpr (f32) x[i] += sc[m][i >> 1][2 + (i & 1)];
+                x[i] = sc[m][i >> 1][i & 1] + sc2[m][i >> 1][i & 1];
+                if constexpr (f32) x[i] += sc[m][i >> 1][2 + (i & 1)] + sc2[m][i >> 1][2 + (i & 1)];
                 x[i] *= factor[m];
                 if (p.cap > 0.0f) x[i] = capped<f32>(x[i], p.cap);
                 x[i] *= 1.44269504088896341f;
@@ -271,6 +302,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             for (int m = 0; m < MT; m++) {
                 const float to = fmaxf(top[m], now[m]), down = to == -INFINITY ? 1.0f : ex2(top[m] - to);
                 top[m] = to;
+                if (u == began) continue;           // (there is nothing yet)
                 sum[m] *= down;
 #pragma unroll
                 for (int i = 0; i < kOut; i++)
@@ -291,21 +323,21 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         {
             const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = lane >> 4;
 #pragma unroll
-            for (int i = 0; i < kOut / 2; i++) {
-                uint32_t b[4];
-                ldsm4_t_at(b, vt + (i >> 2) * (kPsKeys * 128) + r * 128 + (((2 * (i & 3) + c) ^ (r & 7)) << 4));
+            for (int i0 = 0; i0 < kOut / 2; i0 += 4) {
+                uint32_t b[4][4];
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    mma_16<K>(out[m][2 * i], w[m], b[0], b[1]);
-                    mma_16<K>(out[m][2 * i + 1], w[m], b[2], b[3]);
-                }
+                for (int i = 0; i < 4; i++) ldsm4_t_at(b[i], vt + (i0 >> 2) * (kPsKeys * 128) + r * 128 + (((2 * i + c) ^ (r & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        mma_16<K>(out[m][2 * (i0 + i)], w[m], b[i][0], b[i][1]);
+                        mma_16<K>(out[m][2 * (i0 + i) + 1], w[m], b[i][2], b[i][3]);
+                    }
             }
         }
         it.key += kPsKeys;
-        __syncwarp();
-        if (src_u < a1) request(stage);
-
-        if (u + 1 < it.end && u + 1 < a1) continue;
+        if (u + 1 == it.end || u + 1 == a1) {
         // ---- the warp's part of the item is complete
         const bool all = began == it.begin && u + 1 == it.end, tail = u + 1 == a1;
         if (!all) {
@@ -316,7 +348,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const float l = quad_sum(sum[m]);
             const int r = 8 * m + g;
             if (r >= it.job.rows) continue;
-            const int tok = it.job.first + r / p.share, h = it.head * p.share + r % p.share;
+            const int tok = it.job.first + row_tok[m], h = it.head * p.share + row_head[m];
             const size_t row = (size_t)tok * p.heads + h;
             float* dst = nullptr;
             if (all && !it.job.joined) {
@@ -342,84 +374,97 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 #pragma unroll
                 for (int i = 0; i < kOut; i++) store_two<float>(dst + 8 * i + 2 * t4, out[m][i][0] + out[m][i][2], out[m][i][1] + out[m][i][3]);
         }
+        }
+        __syncwarp();
+      }
+      if (src_u < a1) request(stage);
+      if (++stage == kStages) { stage = 0; phase ^= u >= a0; }
     }
+    if (p.mark && warp == kPsWarps - 1) mark_tokens(p, lane, 32, err);
     __syncthreads();
 
-    // ---- items that several warps have parts of
+    // ---- items that several warps have parts of, each row by a warp.  Part e is the first (e even) or last part of warp e / 2.
     constexpr int kCols = DP / 32;
-    int turn = 0;
-    for (int e = 0; e < 2 * kPsWarps;) {
-        const PsPart part = parts[e >> 1][e & 1];
-        if (!part.valid) { e++; continue; }
-        int last = e;                   // entries e .. last: the item's
-        for (int f = e + 1; f < 2 * kPsWarps; f++) {
-            const PsPart& next = parts[f >> 1][f & 1];
-            if (!next.valid) continue;
-            if (next.begin != part.begin) break;
-            last = f;
-        }
-        const bool starts = part.begin >= u0, all = starts && part.end <= u1;
-        for (int r = 0; r < part.rows; r++) {
+    const PsPart* part = &parts[(lane & 15) >> 1][lane & 1];
+    const unsigned exist = __ballot_sync(0xFFFFFFFFu, lane < 2 * kPsWarps && part->valid);
+    const int begins = part->begin, before = exist & ((1u << lane) - 1) ? 31 - __clz(exist & ((1u << lane) - 1)) : lane;
+    const int begins_before = __shfl_sync(0xFFFFFFFFu, begins, before);
+    unsigned heads = __ballot_sync(0xFFFFFFFFu, (exist >> lane & 1u) && (before == lane || begins_before != begins));        // the items' first parts
+    for (int turn = 0; heads;) {
+        const int e = __ffs(heads) - 1;
+        heads &= heads - 1;
+        const unsigned members = exist & ~((1u << e) - 1) & (heads ? (1u << (__ffs(heads) - 1)) - 1 : ~0u);
+        const PsPart item = parts[e >> 1][e & 1];
+        const bool starts = item.begin >= u0, all = starts && item.end <= u1;
+        for (int r = 0; r < item.rows; r++) {
             if (turn++ % kPsWarps != warp) continue;
-            float most = -INFINITY;
-            auto ml = [&](int f) {
-                return f & 1 ? reinterpret_cast<const float2*>(reinterpret_cast<const float*>(ring_ptr + (f >> 1) * kPsRing) + kSplitRows * DP)[r]
-                             : p.head_ml[(size_t)(cta * kPsWarps + (f >> 1)) * kSplitRows + r];
-            };
-            for (int f = e; f <= last; f++)
-                if (parts[f >> 1][f & 1].valid) most = fmaxf(most, ml(f).x);
-            const float base = most == -INFINITY ? 0.0f : most;
-            float acc[kCols], l = 0.0f;
+            // a lane per part: its maximum and sum
+            const int w = (lane & 15) >> 1;
+            float2 v = make_float2(-INFINITY, 0.0f);
+            if (members >> lane & 1u)
+                v = lane & 1 ? reinterpret_cast<const float2*>(reinterpret_cast<const float*>(ring_ptr + w * kPsRing) + kSplitRows * DP)[r]
+                             : p.head_ml[(size_t)(cta * kPsWarps + w) * kSplitRows + r];
+            const float top = warp_max(v.x), weight = ex2(v.x - (top == -INFINITY ? 0.0f : top)), l = warp_sum(weight * v.y);
+            float acc[kCols];
 #pragma unroll
             for (int c = 0; c < kCols; c++) acc[c] = 0.0f;
-            for (int f = e; f <= last; f++) {
-                if (!parts[f >> 1][f & 1].valid) continue;
-                const float2 v = ml(f);
-                const float w = ex2(v.x - base);
-                l = fmaf(w, v.y, l);
-                const float* o = (f & 1 ? reinterpret_cast<const float*>(ring_ptr + (f >> 1) * kPsRing) : p.head_o + (size_t)(cta * kPsWarps + (f >> 1)) * kSplitRows * DP) + r * DP;
+            unsigned rest = members;
+#pragma unroll 1
+            while (rest) {
+                // two parts at a time
+                float x[2][kCols], wi[2];
 #pragma unroll
-                for (int c = 0; c < kCols; c++) acc[c] = fmaf(w, o[kCols * lane + c], acc[c]);
+                for (int k = 0; k < 2; k++) {
+                    const int i = rest ? __ffs(rest) - 1 : 0;
+                    wi[k] = __shfl_sync(0xFFFFFFFFu, weight, i);
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) x[k][c] = 0.0f;
+                    if (rest) {
+                        const float* from = (i & 1 ? reinterpret_cast<const float*>(ring_ptr + (i >> 1) * kPsRing) : p.head_o + (size_t)(cta * kPsWarps + (i >> 1)) * kSplitRows * DP) +
+                                            r * DP + kCols * lane;
+                        if constexpr (kCols == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(from);
+                        else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
+                    }
+                    rest &= rest - 1;
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) acc[c] = fmaf(wi[k], x[k][c], acc[c]);
             }
-            const int tok = part.first + r / p.share, h = part.head * p.share + r % p.share;
+            const int t = r / p.share, tok = item.first + t, h = item.head * p.share + r - t * p.share;
             const size_t row = (size_t)tok * p.heads + h;
-            float* dst = nullptr;
-            float2* dst_ml = nullptr;
-            if (all && !part.joined) {
+            if (all && !item.joined) {
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                A* o = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim;
+                A* out_row = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim;
 #pragma unroll
-                for (int c = 0; c < kCols; c++)
-                    if (kCols * lane + c < p.dim) o[kCols * lane + c] = ActOf<A>::put(acc[c] * inv);
+                for (int c = 0; c < kCols; c += 2)
+                    if (kCols * lane + c < p.dim) store_two<A>(out_row + kCols * lane + c, acc[c] * inv, acc[c + 1] * inv);
             } else {
                 const size_t at = all ? row : (size_t)(2 * cta + starts) * kSplitRows + r;
-                dst = (!all ? p.split_o : (part.prefix ? p.prefix_o : p.own_o)) + at * DP;
-                dst_ml = (!all ? p.split_ml : (part.prefix ? p.prefix_ml : p.own_ml)) + at;
-            }
-            if (dst) {
+                float* dst = (!all ? p.split_o : (item.prefix ? p.prefix_o : p.own_o)) + at * DP + kCols * lane;
 #pragma unroll
-                for (int c = 0; c < kCols; c++) dst[kCols * lane + c] = acc[c];
-                if (lane == 0) *dst_ml = make_float2(most, l);
+                for (int c = 0; c < kCols; c += 2) store_two<float>(dst + c, acc[c], acc[c + 1]);
+                if (lane == 0) (!all ? p.split_ml : (item.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top, l);
             }
             if (lane == 0 && starts) {
                 // the CTA with the item's last unit
-                const int end = all ? cta : (int)(((long long)part.end * ctas - 1) / total);
-                (part.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, r, part.joined && !part.prefix ? kJoinPrefix : 0);
+                const int end = all ? cta : deal.cta_of(item.end - 1);
+                (item.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, r, item.joined && !item.prefix ? kJoinPrefix : 0);
             }
         }
-        e = last + 1;
     }
-    if (p.mark) mark_tokens<kPsThreads>(p, err);
 }
 
 template <typename A, typename K, int DP, int MT>
-static int launch_split(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
+static int launch_split(PagedArgs a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
 {
     CUtensorMap kmap, vmap;
     int rc;
     if ((rc = paged_map(&kmap, kv.k, kv, kPsKeys)) || (rc = paged_map(&vmap, kv.v, kv, kPsKeys))) return rc;
-    if ((rc = allow_smem<k_paged_split<A, K, DP, MT>>(224 * 1024))) return rc;
-    const size_t smem = 1024 + kPsWarps * kPsRing + (size_t)(a.batch + 2 * a.groups + 2) * 4;
+    a.both = paged_both(kv, kPsKeys);
+    if ((rc = allow_smem<k_paged_split<A, K, DP, MT>>(221 * 1024))) return rc;
+    const size_t smem = 1024 + kPsWarps * kPsRing + PagedPlan::size(a);
     return launch_ordered(k_paged_split<A, K, DP, MT>, dim3((unsigned)ctas), kPsThreads, smem, s, kmap, vmap, a, device_error_flag());
 }
 

@@ -112,11 +112,12 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         return n;
     });
     const int ctas = max(1, min((int)gridDim.x, total)), cta = blockIdx.x;
-    const int u0 = cta < ctas ? (int)((long long)total * cta / ctas) : total, u1 = cta < ctas ? (int)((long long)total * (cta + 1) / ctas) : total;
+    const PagedDeal deal(total, ctas);
+    const int u0 = cta < ctas ? deal.first(cta) : total, u1 = cta < ctas ? deal.first(cta + 1) : total;
     auto open = [&](PtItem& it, int u, bool again) {
         if (!again || u >= plan.cum[it.j + 1]) {
             it.j = plan.find(u);
-            it.job = plan.job(p, it.j, err);
+            it.job = plan.known(p, it.j);
         }
         const int per = (plan.cum[it.j + 1] - plan.cum[it.j]) / p.kv_heads;
         int at = u - plan.cum[it.j];
@@ -353,7 +354,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             if (live) {
                 if (!direct) (!all ? p.tile_ml : (it.job.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top, sum);
                 if (starts) {
-                    const int end = all ? cta : (int)(((long long)it.end * ctas - 1) / total);
+                    const int end = all ? cta : deal.cta_of(it.end - 1);
                     (it.job.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, in_part, kJoinTile | (it.job.joined && !it.job.prefix ? kJoinPrefix : 0));
                 }
             }
@@ -406,15 +407,13 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 __syncwarp();
                 const int row = (it.from + b * kPtKeys + lane * box_rows) & (p.page - 1);
                 if (have)
-#pragma unroll
-                    for (int h = 0; h < kHalves; h++)
+                    for (int h = 0; h < (p.both ? 1 : kHalves); h++)
                         tma_page(smem_addr(sk + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), &kmap, 64 * h, row, it.head, now, smem_addr(&k_full[slot]));
                 if (nk >= kDepth && !mbar_wait_bounded(&v_empty[slot], (uint32_t)(nk / kDepth - 1) & 1u, err, 86)) { ok = false; break; }
                 if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
                 __syncwarp();
                 if (have)
-#pragma unroll
-                    for (int h = 0; h < kHalves; h++)
+                    for (int h = 0; h < (p.both ? 1 : kHalves); h++)
                         tma_page(smem_addr(sv + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), &vmap, 64 * h, row, it.head, now, smem_addr(&v_full[slot]));
             }
         }
@@ -474,7 +473,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         __syncwarp();
         }
     }
-    if (p.mark && warp < 4) mark_tokens<128>(p, err);
+    if (p.mark && warp < 4) mark_tokens(p, tid, 128, err);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 1) {
@@ -484,18 +483,19 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 }
 
 template <typename A, typename K, int DP>
-static int launch_tile(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
+static int launch_tile(PagedArgs a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
 {
     CUtensorMap qmap, kmap, vmap;
     int rc;
     if ((rc = paged_map(&kmap, kv.k, kv, kPtKeys)) || (rc = paged_map(&vmap, kv.v, kv, kPtKeys))) return rc;
+    a.both = paged_both(kv, kPtKeys);
     qmap = kmap;                // (of fp32 queries: not used)
     if (sizeof(A) == 2) {
         const int tokens = kPtRows / a.share;
         if ((rc = bf16_map(&qmap, a.q, a.dim, a.heads, a.dim, a.share, a.n_tokens, a.ld_q, tokens))) return rc;
     }
-    if ((rc = allow_smem<k_paged_tile<A, K, DP>>(224 * 1024))) return rc;
-    const size_t smem = 1024 + PtShape<DP>::end + (size_t)(a.batch + 2 * a.groups + 2) * 4;
+    if ((rc = allow_smem<k_paged_tile<A, K, DP>>(221 * 1024))) return rc;
+    const size_t smem = 1024 + PtShape<DP>::end + PagedPlan::size(a);
     return launch_ordered(k_paged_tile<A, K, DP>, dim3((unsigned)ctas), kPtThreads, smem, s, qmap, kmap, vmap, a, device_error_flag());
 }
 

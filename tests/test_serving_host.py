@@ -77,7 +77,7 @@ def test_bad_groups(lib, n, start, pages):
     lib.bpdq_clear_status()
 
 
-@pytest.mark.parametrize("changes", [dict(heads=258, kv_heads=2), dict(batch=2048, max_pages=1 << 21)])
+@pytest.mark.parametrize("changes", [dict(heads=258, kv_heads=2), dict(batch=1280, max_pages=1 << 21), dict(batch=1281)])
 def test_attention_beyond_its_range(lib, changes):
     kv = paged(**changes)
     assert attention(lib, kv, ld_q=258 * 64, ld_o=258 * 64) == -3
