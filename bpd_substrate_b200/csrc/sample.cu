@@ -3,9 +3,9 @@
 // The CTAs of a cluster hold a row between them in shared memory, each a range of the vocabulary, so that it is read once.  A weight
 // w = 2^((x - max) log2(e) / T) is a whole number of 2^-44 (worked out in 64 bits, to 1e-12): sums of 2^18 of them fit 64 bits, are exact, and depend on
 // no order, so neither do the cuts and the choice.  What is kept is always a beginning of the row's order (by value, then by index), hence one
-// place (value, index), the cut.  It is found by a histogram over octaves of weight (32 bins each): the bins that certainly lie above are settled, the few
-// elements of the bin that holds the cut are sorted.  Where those are too many (flat rows, equal values) the bin is halved by exact sums until
-// they are not.
+// place (value, index), the cut.  It is found by a histogram, of numbers over octaves of fp32 weights or of weights over their own leading bits: the bins
+// that certainly lie above are settled, the few elements of the bin that holds the cut are listed in one CTA and compared with each other.  Where
+// those are too many (flat rows, equal values) the bin is halved by exact sums until they are not.
 #include "cluster_device.cuh"
 #include "launch.cuh"
 #include "paged.cuh"
@@ -13,8 +13,8 @@
 namespace bpdq {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 2048, kSampleOctave = 32;       // bins, bins per octave of weight: 64 octaves, far more than a weight has bits
-constexpr int kSampleOctaves = kSampleBins / kSampleOctave;
+constexpr int kCountBins = 2048, kCountOctave = 32;         // numbers: bins, bins per octave of weight
+constexpr int kMassBins = 5888, kMassOctave = 128;          // weights: the 46 octaves down to 2^-45
 constexpr int kSampleList = 1024;                           // elements that are sorted
 constexpr int kSampleCounted = 256;                         // elements that are compared with each other instead
 constexpr int kSampleBits = 44;
@@ -34,12 +34,12 @@ struct SampleArgs {
 struct SampleShared {
     u64 list[kSampleList];                                  // places
     u64 weight[kSampleList];
-    unsigned hist[kSampleBins];
-    double octave[kSampleOctaves];
+    unsigned hist[kMassBins];
+    double octave[64];
     u64 red[2][2], warp_red[kSampleWarps][2], warp_sum[kSampleWarps];
     unsigned exp_lo[32], exp_hi[32];
     unsigned list_n, found[4], least, most;
-    double before;
+    float from, to;
     u64 answer[3];
 };
 
@@ -67,12 +67,6 @@ __device__ __forceinline__ unsigned peer_u32(const unsigned* p, uint32_t rank)
     return v;
 }
 __device__ __forceinline__ double peer_f64(const double* p, uint32_t rank) { return __longlong_as_double((long long)peer_u64(reinterpret_cast<const u64*>(p), rank)); }
-__device__ __forceinline__ unsigned peer_add(unsigned* p, uint32_t rank, unsigned v)
-{
-    unsigned old;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(peer_addr(p, rank)), "r"(v) : "memory");
-    return old;
-}
 __device__ __forceinline__ void peer_store_u64(u64* p, uint32_t rank, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(p, rank)), "l"(v) : "memory"); }
 __device__ __forceinline__ void cluster_meet() { cluster_arrive(); cluster_wait(); }
 
@@ -100,6 +94,15 @@ __device__ __forceinline__ u64 warp_total(u64 v)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ u64 warp_most(u64 v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 t = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        if (t > v) v = t;
+    }
     return v;
 }
 template <typename T> __device__ __forceinline__ T warp_scan(T v, int lane)
@@ -143,16 +146,16 @@ struct Sampler {
     float top, rate;                // the largest logit; log2(e) / T
     double top64, rate64;
     u64 cut;                        // places >= cut are kept
+    bool whole;                     // they all are
     int meetings;
 
-    // In octaves below the largest; falls with x.
-    __device__ __forceinline__ float octaves(float v) const { return v == top ? 0.0f : (top - v) * rate; }
-    __device__ __forceinline__ int bin_of(float v) const { return (int)fminf(octaves(v) * (float)kSampleOctave, (float)(kSampleBins - 1)); }
-    // 2^44 2^y, y = (v - top) log2(e) / T: y = j / 32 + f, |f| <= 1/64, a table for j and the Taylor polynomial of degree 5 of 2^f (remainder 3e-15).  Without branches: several
+    // fp32 octaves below the largest, as bins; rise as v falls.
+    __device__ __forceinline__ int bin_of(float v) const { return (int)fminf((top - v) * rate * (float)kCountOctave, (float)(kCountBins - 1)); }
+    // 2^44 2^y, y = (v - top) log2(e) / T = j / 32 + f, |f| <= 1/64: a table for j and the Taylor polynomial of degree 5 of 2^f (remainder 3e-15).  Without branches: several
     // of them run side by side.
-    __device__ __forceinline__ u64 weight(float v) const
+    __device__ __forceinline__ double scaled(float v) const
     {
-        const double y = fmax(((double)v - top64) * rate64, -60.0);         // (NaN, beside infinity: nothing)
+        const double d = ((double)v - top64) * rate64, y = d > -60.0 ? d : -60.0;         // (weights have long been 0 there)
         const double shift = 6755399441055744.0 / 32.0;             // 1.5 2^52 / 32: the sum's last bit is 1/32
         const double k = y + shift, f = y - (k - shift);
         const int j = __double2loint(k);
@@ -162,10 +165,11 @@ struct Sampler {
         p = fma(p, f, 0.24022650695910071);
         p = fma(p, f, 0.69314718055994531);
         p = fma(p, f, 1.0);
-        const double t = __hiloint2double((int)s.exp_hi[j & 31] + ((j >> 5) + kSampleBits) * (1 << 20), (int)s.exp_lo[j & 31]);      // 2^44 2^(j / 32)
-        const u64 w = (u64)(__double_as_longlong(fma(p, t, 4503599627370496.0)) & 0xFFFFFFFFFFFFFll);       // to the nearest whole number
-        return v == top ? 1ull << kSampleBits : w;
+        return p * __hiloint2double((int)s.exp_hi[j & 31] + ((j >> 5) + kSampleBits) * (1 << 20), (int)s.exp_lo[j & 31]);      // 2^44 2^(j / 32)
     }
+    // To the nearest whole number.
+    static __device__ __forceinline__ u64 whole_of(double z) { return (u64)(__double_as_longlong(z + 4503599627370496.0) & 0xFFFFFFFFFFFFFll); }
+    __device__ __forceinline__ u64 weight(float v) const { return whole_of(scaled(v)); }
     __device__ __forceinline__ bool kept(float v, int i) const { return place_of(v, i) >= cut; }
     // f(four neighbouring values, index of the first) for the warp's elements, 128 at a time in the order of the vocabulary, all lanes together.
     template <class F> __device__ __forceinline__ void each(F f) const
@@ -191,61 +195,135 @@ struct Sampler {
             if (lane == 0) red[warp] = v;
         }
         cluster_meet();
-        a = b = 0;
-#pragma unroll 1
-        for (uint32_t r = 0; r < ranks; r++) { a += peer_u64(&red[0], r); b += peer_u64(&red[1], r); }
+        a = warp_total(lane < ranks ? peer_u64(&red[0], lane) : 0);
+        b = warp_total(lane < ranks ? peer_u64(&red[1], lane) : 0);
         meetings++;
     }
 
-    // Of the histogram's octaves, the sums of this CTA (of weights: in units of theirs).
-    __device__ __forceinline__ void sum_octaves(bool mass)
+    // The histogram's weights are multiples of 2^-15 of their octave's smallest.
+    static __device__ __forceinline__ double unit_of(int octave) { return __hiloint2double((1023 + kSampleBits - 15 - octave) << 20, 0); }
+    // This CTA's sums of the histogram's octaves.
+    template <bool kMass> __device__ __forceinline__ void sum_octaves()
     {
         __syncthreads();
-        static_assert(kSampleThreads * 4 == kSampleBins && kSampleOctave == 32, "eight threads per octave");
-        const uint4 h = reinterpret_cast<const uint4*>(s.hist)[tid];
-        u64 v = (u64)h.x + h.y + h.z + h.w;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        if ((tid & 7) == 0) s.octave[tid >> 3] = (double)v * (mass ? unit_of(tid >> 3) : 1.0);
+        constexpr int octaves = kMass ? kMassBins / kMassOctave : kCountBins / kCountOctave;
+        for (int o = warp; o < 64; o += kSampleWarps) {
+            double v = 0.0;
+            if (o < octaves) {
+                if constexpr (kMass) {
+                    const uint4 h = reinterpret_cast<const uint4*>(s.hist)[o * 32 + lane];
+                    v = (double)warp_total((u64)h.x + h.y + h.z + h.w) * unit_of(o);
+                } else {
+                    v = (double)__reduce_add_sync(0xFFFFFFFFu, s.hist[o * 32 + lane]);
+                }
+            }
+            if (lane == 0) s.octave[o] = v;
+        }
     }
-    // The histogram's weights are multiples of 2^-16 of their octave's largest.
-    static __device__ __forceinline__ double unit_of(int octave) { return __hiloint2double((1023 + kSampleBits - 16 - octave) << 20, 0); }
-    // Walks the merged histogram, octave by octave and then bin by bin (warp 0; after a meeting): the first bin b for which reached(sum up to b, sum of all) holds, or
-    // kSampleBins; the sum ahead of it.
-    template <class R> __device__ __forceinline__ int first_bin(bool mass, R reached, double& before) const
+    // The histogram of the cluster (a warp, after a meeting): octave by octave, then bin by bin.
+    struct Octaves { double two[2], up, all; };              // of octaves 2 lane and 2 lane + 1; sum up to them; sum of all
+    __device__ __forceinline__ Octaves octaves() const
     {
-        double o[2] = {0.0, 0.0};
-#pragma unroll 1
-        for (uint32_t r = 0; r < ranks; r++)
+        Octaves o = {{0.0, 0.0}, 0.0, 0.0};
 #pragma unroll
-            for (int i = 0; i < 2; i++) o[i] += peer_f64(&s.octave[2 * lane + i], r);
-        const double up = warp_scan(o[0] + o[1], lane), all = __shfl_sync(0xFFFFFFFFu, up, 31);
-        const unsigned who0 = __ballot_sync(0xFFFFFFFFu, reached(up - o[1], all)), who1 = __ballot_sync(0xFFFFFFFFu, reached(up, all));
-        before = all;
-        if (!(who0 | who1)) return kSampleBins;
-        // octave 2 l is reached first where lane l is the first in who0 and none ahead of it is in who1
-        const int l0 = who0 ? __ffs(who0) - 1 : 32, l1 = who1 ? __ffs(who1) - 1 : 32, lead = min(l0, l1);
-        const int octave = 2 * lead + (l0 <= l1 ? 0 : 1);
-        const double ahead = __shfl_sync(0xFFFFFFFFu, up - o[1] - (l0 <= l1 ? o[0] : 0.0), lead);
-        u64 h = 0;
-#pragma unroll 1
-        for (uint32_t r = 0; r < ranks; r++) h += peer_u32(&s.hist[32 * octave + lane], r);
-        const double mine = (double)h * (mass ? unit_of(octave) : 1.0), run = ahead + warp_scan(mine, lane);
-        const unsigned who = __ballot_sync(0xFFFFFFFFu, reached(run, all));
-        const int b = who ? __ffs(who) - 1 : 31;
-        before = __shfl_sync(0xFFFFFFFFu, run - mine, b);
-        return 32 * octave + b;
+        for (int r = 0; r < 8; r++)
+            if (r < (int)ranks) {
+                o.two[0] += peer_f64(&s.octave[2 * lane], r);
+                o.two[1] += peer_f64(&s.octave[2 * lane + 1], r);
+            }
+        o.up = warp_scan(o.two[0] + o.two[1], lane);
+        o.all = __shfl_sync(0xFFFFFFFFu, o.up, 31);
+        return o;
+    }
+    // The first bin b for which reached(sum up to b) holds, or -1; the sum ahead of it, and what it holds.
+    template <bool kMass, class R> __device__ __forceinline__ int first_bin(const Octaves& o, R reached, double& before, double& holds) const
+    {
+        constexpr int n = (kMass ? kMassOctave : kCountOctave) / 32;
+        const unsigned who0 = __ballot_sync(0xFFFFFFFFu, reached(o.up - o.two[1])), who1 = __ballot_sync(0xFFFFFFFFu, reached(o.up));
+        before = o.all;
+        holds = 0.0;
+        if (!(who0 | who1)) return -1;
+        const int l0 = who0 ? __ffs(who0) - 1 : 32, l1 = who1 ? __ffs(who1) - 1 : 32, lead = min(l0, l1), octave = 2 * lead + (l0 <= l1 ? 0 : 1);
+        double run = __shfl_sync(0xFFFFFFFFu, o.up - o.two[1] - (l0 <= l1 ? o.two[0] : 0.0), lead);
+        u64 h[n];
+#pragma unroll
+        for (int i = 0; i < n; i++) h[i] = 0;
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            if (r < (int)ranks)
+#pragma unroll
+                for (int i = 0; i < n; i++) h[i] += peer_u32(&s.hist[32 * n * octave + n * lane + i], r);
+        u64 mine = 0;
+#pragma unroll
+        for (int i = 0; i < n; i++) mine += h[i];
+        const double unit = kMass ? unit_of(octave) : 1.0;
+        run += (double)(warp_scan(mine, lane) - mine) * unit;
+        int at = n;
+        double sum = run;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            sum += (double)h[i] * unit;
+            if (at == n && reached(sum)) at = i;
+        }
+        const unsigned who = __ballot_sync(0xFFFFFFFFu, at < n);
+        const int l = who ? __ffs(who) - 1 : 31;
+        if (at == n) at = n - 1;            // (sums in another order: the octave's last bin)
+        double mine_before = run, mine_holds = 0.0;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            if (i < at) mine_before += (double)h[i] * unit;
+            if (i == at) mine_holds = (double)h[i] * unit;
+        }
+        before = __shfl_sync(0xFFFFFFFFu, mine_before, l);
+        holds = __shfl_sync(0xFFFFFFFFu, mine_holds, l);
+        return 32 * n * octave + n * l + __shfl_sync(0xFFFFFFFFu, at, l);
     }
 
-    // Puts the place where `yes` holds into rank 0's list, while there is room; list_n counts them all.
+    // Puts the place where `yes` holds into this CTA's list, while there is room; list_n counts them all.
     __device__ __forceinline__ void list_if(bool yes, u64 place) const
     {
         const unsigned who = __ballot_sync(0xFFFFFFFFu, yes);
         if (!who) return;
         unsigned at = 0;
-        if (lane == 0) at = peer_add(&s.list_n, 0, __popc(who));
+        if (lane == 0) at = atomicAdd(&s.list_n, __popc(who));
         at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(who & ((1u << lane) - 1));
-        if (yes && at < kSampleList) peer_store_u64(&s.list[at], 0, place);
+        if (yes && at < kSampleList) s.list[at] = place;
+    }
+    // Of the CTAs' lists (after a meeting): how many places they hold.
+    __device__ __forceinline__ unsigned listed() const { return __reduce_add_sync(0xFFFFFFFFu, lane < ranks ? peer_u32(&s.list_n, lane) : 0u); }
+    // Rank 0 appends the others' lists to its own; up to kSampleList places in all.
+    __device__ __forceinline__ void collect()
+    {
+        const unsigned n = lane < ranks ? peer_u32(&s.list_n, lane) : 0u, ahead = warp_scan(n, lane) - n;
+        const uint32_t r = (uint32_t)warp & (ranks - 1);
+        const unsigned from = __shfl_sync(0xFFFFFFFFu, ahead, r), count = __shfl_sync(0xFFFFFFFFu, n, r);
+        if (r > 0)
+            for (unsigned i = 32 * (warp / ranks) + lane; i < count; i += 32 * (kSampleWarps / ranks)) s.list[from + i] = peer_u64(&s.list[i], r);
+        __syncthreads();
+    }
+    // For listed element tid / parts of n <= kSampleCounted: how many of the others lie ahead of it, and the sum of their s.weight; in all of its threads, of
+    // which there are `parts`, neighbours.
+    __device__ __forceinline__ void counted(int n, int parts, int& ahead, u64& mass) const
+    {
+        const int j = tid / parts;
+        ahead = 0;
+        mass = 0;
+        if (j < n) {
+            const u64 mine = s.list[j];
+#pragma unroll 2
+            for (int i = tid & (parts - 1); i < n; i += parts)
+                if (s.list[i] > mine) { ahead++; mass += s.weight[i]; }
+        }
+        for (int o = parts / 2; o > 0; o >>= 1) {
+            ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, o);
+            mass += __shfl_xor_sync(0xFFFFFFFFu, mass, o);
+        }
+    }
+    static __device__ __forceinline__ int parts_for(int n)
+    {
+        int parts = 2;
+        while (parts < 32 && 2 * parts * n <= kSampleThreads) parts *= 2;
+        return parts;
     }
 
     // s.weight[i] = sum of f(0) .. f(i), i < n <= 1024.
@@ -285,22 +363,20 @@ struct Sampler {
         return v;
     }
 
-    // Sums of this thread's warp's and CTA's predecessors, in the vocabulary's order, over the cluster; sum: of the warp.  One meeting.
-    __device__ __forceinline__ u64 ahead_of_warp(u64 mine, u64& sum)
+    // Sums of this thread's warp's and CTA's predecessors, in the vocabulary's order, over the cluster; sum: of the warp; all: of the cluster.  One meeting.
+    __device__ __forceinline__ u64 ahead_of_warp(u64 mine, u64& sum, u64& all)
     {
         sum = warp_total(mine);
         if (lane == 0) s.warp_sum[warp] = sum;
         __syncthreads();
-        u64 before = 0, cta = 0;
-#pragma unroll 1
-        for (int w = 0; w < kSampleWarps; w++) {
-            if (w < warp) before += s.warp_sum[w];
-            cta += s.warp_sum[w];
-        }
+        const u64 of = lane < kSampleWarps ? s.warp_sum[lane] : 0;
+        u64 before = warp_total(lane < warp ? of : 0);
+        const u64 cta = warp_total(of);
         if (tid == 0) s.answer[0] = cta;
         cluster_meet();
-#pragma unroll 1
-        for (uint32_t r = 0; r < rank; r++) before += peer_u64(&s.answer[0], r);
+        const u64 peer = lane < ranks ? peer_u64(&s.answer[0], lane) : 0;
+        before += warp_total(lane < rank ? peer : 0);
+        all = warp_total(peer);
         return before;
     }
     // found(place) in the lane that holds the first element at which the sum of f, `run` ahead of the warp, reaches want.
@@ -360,12 +436,12 @@ __device__ __forceinline__ bool narrow(Sampler& w, Border& b)
     const float v = value_of(b.lo);
     const u64 each_one = one(v), nth = each_one ? (b.want - b.above + each_one - 1) / each_one : 1;
     auto equal = [&](float a, int i) -> u64 { return a == v && w.kept(a, i); };
-    u64 mine = 0, sum;
+    u64 mine = 0, sum, all;
     w.each([&](const float (&a)[4], int i) {
 #pragma unroll 1
         for (int j = 0; j < 4; j++) mine += equal(a[j], i + j);
     });
-    const u64 run = w.ahead_of_warp(mine, sum);
+    const u64 run = w.ahead_of_warp(mine, sum, all);
     if (run < nth && nth <= run + sum)
         w.walk(run, nth, equal, [&](u64 place) {
 #pragma unroll 1
@@ -376,20 +452,36 @@ __device__ __forceinline__ bool narrow(Sampler& w, Border& b)
     return true;
 }
 
-// The cut among the border's elements, which are listed in rank 0.  All threads of the cluster.
+// The cut among the border's elements, which the CTAs have listed (after a meeting).  All threads of the cluster.
 template <bool kMass>
 __device__ __forceinline__ void cut_in_list(Sampler& w, const Border& b)
 {
     if (w.rank == 0) {
         const int n = (int)b.count;
-        sort_list(w.s.list, n, w.tid);
-        w.scan_weights(n, [&](int i) -> u64 { return kMass ? w.weight(place_value(w.s.list[i])) : 1; });
-        const int at = w.first_reaching(n, b.want - b.above);
-        if (w.tid < (int)w.ranks) peer_store_u64(&w.s.answer[2], (uint32_t)w.tid, w.s.list[at < n ? at : n - 1]);
-        if (w.tid == 0) w.s.list_n = 0;
+        SampleShared& s = w.s;
+        w.collect();
+        auto one = [&](u64 place) -> u64 { return kMass ? w.weight(place_value(place)) : 1; };
+        if (n <= kSampleCounted) {
+            if (w.tid < n) s.weight[w.tid] = one(s.list[w.tid]);
+            __syncthreads();
+            const int parts = Sampler::parts_for(n), j = w.tid / parts;
+            int ahead;
+            u64 mass;
+            w.counted(n, parts, ahead, mass);
+            // the element that reaches the sum (the last one, should none)
+            if (j < n && b.above + mass < b.want && (b.above + mass + s.weight[j] >= b.want || ahead == n - 1))
+                for (int r = w.tid & (parts - 1); r < (int)w.ranks; r += parts) peer_store_u64(&s.answer[2], (uint32_t)r, s.list[j]);
+        } else {
+            sort_list(s.list, n, w.tid);
+            w.scan_weights(n, [&](int i) -> u64 { return one(s.list[i]); });
+            const int at = w.first_reaching(n, b.want - b.above);
+            if (w.tid < (int)w.ranks) peer_store_u64(&s.answer[2], (uint32_t)w.tid, s.list[at < n ? at : n - 1]);
+        }
     }
     cluster_meet();
+    if (w.tid == 0) w.s.list_n = 0;
     w.cut = w.s.answer[2];
+    w.whole = false;
 }
 // Lists the border's elements (list_n is 0), then as above.
 template <bool kMass>
@@ -399,7 +491,7 @@ __device__ __noinline__ u64 cut_at_border(Sampler w, Border b, int& meetings)
     meetings = w.meetings;
     if (known) return w.cut;
     w.each([&](const float (&v)[4], int i) {
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < 4; j++) {
             const unsigned k = order_of(v[j]);
             w.list_if(k >= b.lo && k <= b.hi && w.kept(v[j], i + j), place_of(v[j], i + j));
@@ -430,7 +522,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
         s.exp_hi[tid] = (unsigned)__double2hiint(t);
     }
     if (tid == 0) { s.list_n = 0; s.least = 0xFFFFFFFFu; s.most = 0; }
-    reinterpret_cast<uint4*>(s.hist)[tid] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < kMassBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
     pdl_wait();
     pdl_launch_dependents();
 
@@ -464,29 +556,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
     for (int i = n + tid; i < kSampleWarps * w.chunk; i += kSampleThreads) x[i] = -INFINITY;
     u64 first = place_of(best, w.base + best_at);
     if (best == -INFINITY) first = 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 other = __shfl_xor_sync(0xFFFFFFFFu, first, o);
-        if (other > first) first = other;
-    }
+    first = warp_most(first);
     if (lane == 0) s.warp_sum[warp] = first;
     __syncthreads();
     if (warp == 0) {
-        first = s.warp_sum[lane & (kSampleWarps - 1)];
-#pragma unroll
-        for (int o = kSampleWarps / 2; o > 0; o >>= 1) {
-            const u64 other = __shfl_xor_sync(0xFFFFFFFFu, first, o);
-            if (other > first) first = other;
-        }
+        first = warp_most(lane < kSampleWarps ? s.warp_sum[lane] : 0);
         if (lane == 0) s.answer[1] = first;
     }
     cluster_meet();
-    first = 0;
-#pragma unroll 1
-    for (uint32_t r = 0; r < w.ranks; r++) {
-        const u64 other = peer_u64(&s.answer[1], r);
-        if (other > first) first = other;
-    }
+    first = warp_most(lane < w.ranks ? peer_u64(&s.answer[1], lane) : 0);
     cluster_arrive();                                            // (answer[1] is not written again; nobody leaves before all have read)
     const bool lead = w.rank == 0 && tid == 0, none = first == 0;
     if (none || !(temperature > 0.0f)) {
@@ -498,20 +576,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
         return;
     }
     w.top = place_value(first);
+    if (w.top == INFINITY) {
+        // infinite logits share everything: as 0 beside -inf
+        for (int i = tid; i < kSampleWarps * w.chunk; i += kSampleThreads) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+        w.top = 0.0f;
+        __syncthreads();
+    }
+    // beyond this temperature all logits but the lowest numbers of fp32 weigh the same
+    const float warm = fminf(temperature, 8e36f);
     w.top64 = (double)w.top;
-    w.rate64 = kLog2e / (double)temperature;
-    w.rate = (float)w.rate64;
+    w.rate64 = kLog2e / (double)warm;
+    w.rate = fminf((float)w.rate64, 3e38f);
     w.cut = place_of(-INFINITY, -1) + 1;                         // everything but -inf
+    w.whole = true;
     const bool cut_k = k > 0 && k < p.vocab, cut_p = part < 1.0f, cut_m = least > 0.0f;
     // the least logit with w >= min_p, w rounded to 64 bits (1 - 2^-54 is 1)
     float floor_m = -INFINITY;
-    if (cut_m && w.top < INFINITY && w.rate64 > 0.0) {           // (otherwise weights are 1 and 0, or all 1)
+    if (cut_m) {
         floor_m = __double2float_ru(w.top64 + (log2((double)least) - kLog2e / 18014398509481984.0) / w.rate64);
         if (!(floor_m <= w.top)) floor_m = w.top;
     }
     auto answer = [&](float v, int i, u64 all) {
         p.token[row] = i;
-        if (p.logprob) p.logprob[row] = (float)((v == w.top ? 0.0 : ((double)v - w.top64) / (double)temperature) - log((double)all * (1.0 / (double)(1ull << kSampleBits))));
+        if (p.logprob) p.logprob[row] = (float)(((double)v - w.top64) / (double)warm - log((double)all * (1.0 / (double)(1ull << kSampleBits))));
     };
     cluster_wait();
 
@@ -521,57 +608,56 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             for (int j = 0; j < 4; j++)
                 if (v[j] > -INFINITY) atomicAdd(&s.hist[w.bin_of(v[j])], 1u);
         });
-        w.sum_octaves(false);
+        w.sum_octaves<false>();
         cluster_meet();
         if (warp == 0) {
-            double before;
-            const int b = w.first_bin(false, [&](double up, double) { return up >= (double)k; }, before);
+            double before, holds;
+            const int b = w.first_bin<false>(w.octaves(), [&](double up) { return up >= (double)k; }, before, holds);
             // elements in bins up to it (all, where there are fewer than k)
-            unsigned in_bin = 0;
-            if (b < kSampleBins)
-#pragma unroll 1
-                for (uint32_t r = 0; r < w.ranks; r++) in_bin += peer_u32(&s.hist[b], r);
-            if (lane == 0) { s.found[1] = (unsigned)b; s.found[2] = (unsigned)before; s.found[3] = in_bin; }
+            if (lane == 0) { s.found[1] = (unsigned)(b < 0 ? kCountBins : b); s.found[2] = (unsigned)before; s.found[3] = (unsigned)holds; }
         }
         __syncthreads();
         const int b = (int)s.found[1], above = (int)s.found[2], in_bin = (int)s.found[3];
         if (above + in_bin <= kSampleList) {
             // ---- few enough for one CTA to finish
             w.each([&](const float (&v)[4], int i) {
-                // one vote for four: most have none
-                const bool any = (v[0] > -INFINITY && w.bin_of(v[0]) <= b) || (v[1] > -INFINITY && w.bin_of(v[1]) <= b) || (v[2] > -INFINITY && w.bin_of(v[2]) <= b) ||
-                                 (v[3] > -INFINITY && w.bin_of(v[3]) <= b);
-                if (!__any_sync(0xFFFFFFFFu, any)) return;
+                bool in[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) w.list_if(v[j] > -INFINITY && w.bin_of(v[j]) <= b, place_of(v[j], i + j));
+                for (int j = 0; j < 4; j++) in[j] = v[j] > -INFINITY && w.bin_of(v[j]) <= b;
+                if (!__any_sync(0xFFFFFFFFu, in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll 1
+                for (int j = 0; j < 4; j++) w.list_if(in[j], place_of(v[j], i + j));
             });
             cluster_meet();
-            if (w.rank != 0) return;
+            if (w.rank != 0) {
+                cluster_meet();                                  // until rank 0 has the list
+                return;
+            }
+            w.collect();
+            cluster_meet();
             const int n = above + in_bin;
             if (n <= kSampleCounted) {
                 // An element is kept if fewer than k and less than the share of top_p lie ahead of it: both counted from the list as it is.
-                const u64 mine = tid < n ? s.list[tid] : 0, wt = tid < n ? w.weight(place_value(mine)) : 0;
-                if (tid < n) s.weight[tid] = wt;
+                const int parts = Sampler::parts_for(n), j = tid / parts;
+                if (tid < n) s.weight[tid] = w.weight(place_value(s.list[tid]));
                 __syncthreads();
-                int ahead = 0;
-                u64 mass = 0;
-                if (tid < n)
-#pragma unroll 4
-                    for (int i = 0; i < n; i++)
-                        if (s.list[i] > mine) { ahead++; mass += s.weight[i]; }
-                const bool in_k = tid < n && ahead < k;
-                const u64 all_k = w.cta_total(in_k ? wt : 0);
+                const u64 mine = j < n ? s.list[j] : 0, wt = j < n ? s.weight[j] : 0;
+                int ahead;
+                u64 mass;
+                w.counted(n, parts, ahead, mass);
+                const bool lead = (tid & (parts - 1)) == 0, in_k = j < n && ahead < k;
+                const u64 all_k = w.cta_total(lead && in_k ? wt : 0);
                 const u64 want = cut_p ? (u64)fmax(ceil((double)part * (double)all_k), 1.0) : ~0ull;
                 const bool keep = in_k && mass < want && place_value(mine) >= floor_m;
-                if (tid < n) s.weight[tid] = keep ? wt : 0;
-                const u64 sum = w.cta_total(keep ? wt : 0), goal = (u64)(u * (double)sum) + 1;
-                u64 upto = 0;
-                if (keep) {
-#pragma unroll 4
-                    for (int i = 0; i < n; i++)
-                        if ((unsigned)s.list[i] >= (unsigned)mine) upto += s.weight[i];           // indices up to its own
-                    if (upto >= goal && upto - wt < goal) answer(place_value(mine), place_index(mine), sum);
-                }
+                if (lead && j < n) s.weight[j] = keep ? wt : 0;
+                const u64 sum = w.cta_total(lead && keep ? wt : 0), goal = (u64)(u * (double)sum) + 1;
+                u64 upto = 0;                                    // of indices up to its own
+                if (keep)
+#pragma unroll 2
+                    for (int i = tid & (parts - 1); i < n; i += parts)
+                        if ((unsigned)s.list[i] >= (unsigned)mine) upto += s.weight[i];
+                for (int o = parts / 2; o > 0; o >>= 1) upto += __shfl_xor_sync(0xFFFFFFFFu, upto, o);
+                if (lead && keep && upto >= goal && upto - wt < goal) answer(place_value(mine), place_index(mine), sum);
                 return;
             }
             sort_list(s.list, n, tid);
@@ -611,7 +697,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             }
             return;
         }
-        if (b < kSampleBins) {
+        if (b < kCountBins) {
             // the bin's keys, then its elements
             unsigned lo = 0xFFFFFFFFu, hi = 0;
             w.each([&](const float (&v)[4], int) {
@@ -623,15 +709,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             hi = __reduce_max_sync(0xFFFFFFFFu, hi);
             if (lane == 0) { atomicMin(&s.least, lo); atomicMax(&s.most, hi); }
             cluster_meet();
-#pragma unroll 1
-            for (uint32_t r = 0; r < w.ranks; r++) { lo = min(lo, peer_u32(&s.least, r)); hi = max(hi, peer_u32(&s.most, r)); }
+            lo = __reduce_min_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.least, lane) : 0xFFFFFFFFu);
+            hi = __reduce_max_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.most, lane) : 0u);
             int meetings;
             w.cut = cut_at_border<false>(w, Border{lo, hi, (u64)in_bin, (u64)above, (u64)k}, meetings);
             w.meetings = meetings;
+            w.whole = false;
         }
         if (cut_p) {
             cluster_meet();                                      // (the histogram and the bounds are still being read)
-            reinterpret_cast<uint4*>(s.hist)[tid] = make_uint4(0, 0, 0, 0);
+            for (int i = tid; i < kMassBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
             if (tid == 0) { s.least = 0xFFFFFFFFu; s.most = 0; }
             __syncthreads();
         }
@@ -641,32 +728,40 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
     unsigned lo = 0, hi = 0xFFFFFFFFu;                           // keys of elements that are not in it yet
     if (cut_p) {
         u64 sum = 0, nothing = 0;
-        // per bin, the weights as multiples of 2^-16 of its octave's, rounded up: within 2^-14 of the bin's sum, errors of fp32 octaves included
+        // per bin, of the weights' leading bits, what they begin with in multiples of 2^-15, rounded up: within 2^-14 of the bin's sum
+        constexpr int first_key = ((1023 + kSampleBits) << 7) + 127;
         w.each([&](const float (&v)[4], int i) {
-            bool in[4];
-            u64 wt[4];
+            double z[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) { in[j] = w.kept(v[j], i + j); wt[j] = w.weight(v[j]); }
+            for (int j = 0; j < 4; j++) z[j] = w.scaled(v[j]);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float d = w.octaves(v[j]);
-                if (in[j]) sum += wt[j];
-                if (in[j] && d < (float)kSampleOctaves) atomicAdd(&s.hist[(int)(d * (float)kSampleOctave)], (unsigned)(ex2(floorf(d) - d) * 65536.0f) + 1u);
+                if (!w.whole && !w.kept(v[j], i + j)) z[j] = 0.0;
+                sum += Sampler::whole_of(z[j]);
+                const int hi = __double2hiint(z[j]), b = first_key - (hi >> 13);
+                if (b < kMassBins) atomicAdd(&s.hist[b], ((unsigned)((hi & 0xFFFFF) | 0x100000) >> 5) + 1u);
             }
         });
-        w.sum_octaves(true);
+        w.sum_octaves<true>();
         w.total(sum, nothing);
         const u64 want = (u64)fmax(ceil((double)part * (double)sum), 1.0);
         if (warp == 0) {
             // the sum up to a bin from either side: whichever is less is known better
             const double m = (double)sum, goal = (double)want, slack = (double)p.vocab, err = 1.0 / 16384.0;
-            double before;
-            const int b1 = w.first_bin(true, [&](double up, double all) { return fmin(up * (1.0 + err), m - fmax(all - up, 0.0) * (1.0 - err)) + slack >= goal; }, before);
-            const int b2 = w.first_bin(true, [&](double up, double all) { return fmax(up * (1.0 - err), m - fmax(all - up, 0.0) * (1.0 + err)) - slack >= goal; }, before);
-            if (lane == 0) { s.found[1] = (unsigned)min(b1, kSampleBins - 1); s.found[2] = (unsigned)min(b2, kSampleBins - 1); }
+            const typename Sampler::Octaves o = w.octaves();
+            double before, holds;
+            const int b1 = w.first_bin<true>(o, [&](double up) { return fmin(up * (1.0 + err), m - fmax(o.all - up, 0.0) * (1.0 - err)) + slack >= goal; }, before, holds);
+            const int b2 = w.first_bin<true>(o, [&](double up) { return fmax(up * (1.0 - err), m - fmax(o.all - up, 0.0) * (1.0 + err)) - slack >= goal; }, before, holds);
+            // the logits at the ends of bins b1 .. b2, and 1e-13 octaves beyond, which weights are not off by
+            if (lane < 2) {
+                const int bin = lane == 0 ? b1 : b2, key = first_key - bin + (lane == 0 ? 1 : 0);
+                const double at = w.top64 + (log2(__hiloint2double(key << 13, 0)) - (double)kSampleBits + (lane == 0 ? 1e-13 : -1e-13)) / w.rate64;
+                if (lane == 0) s.to = bin < 0 ? -INFINITY : __double2float_ru(at);
+                else s.from = bin < 0 ? -INFINITY : __double2float_rd(at);
+            }
         }
         __syncthreads();
-        const int b1 = (int)s.found[1], b2 = (int)s.found[2];
+        const float from = s.from, to = s.to;
         // the exact sum above, and the elements of the bins with the cut
         u64 above = 0;
         lo = 0xFFFFFFFFu;
@@ -675,20 +770,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             bool over[4], in[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int b = w.bin_of(v[j]);
-                const bool yes = w.kept(v[j], i + j);
-                over[j] = yes && b < b1;
-                in[j] = yes && b >= b1 && b <= b2;
+                const bool yes = v[j] > -INFINITY && (w.whole || w.kept(v[j], i + j));
+                over[j] = yes && v[j] > to;
+                in[j] = yes && v[j] <= to && v[j] >= from;
             }
             if (__any_sync(0xFFFFFFFFu, over[0] || over[1] || over[2] || over[3])) {
+                u64 wt[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) wt[j] = w.weight(v[j]);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const u64 wt = w.weight(v[j]);
-                    if (over[j]) { above += wt; if (v[j] >= floor_m) mine += wt; }
+                    above += over[j] ? wt[j] : 0;
+                    mine += over[j] && v[j] >= floor_m ? wt[j] : 0;
                 }
             }
             if (__any_sync(0xFFFFFFFFu, in[0] || in[1] || in[2] || in[3])) {
-#pragma unroll
+#pragma unroll 1
                 for (int j = 0; j < 4; j++) {
                     if (in[j]) { lo = min(lo, order_of(v[j])); hi = max(hi, order_of(v[j])); }
                     w.list_if(in[j], place_of(v[j], i + j));
@@ -699,19 +796,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
         hi = __reduce_max_sync(0xFFFFFFFFu, hi);
         if (lane == 0) { atomicMin(&s.least, lo); atomicMax(&s.most, hi); }
         w.total(above, nothing);
-        Border b = {0xFFFFFFFFu, 0, (u64)peer_u32(&s.list_n, 0), above, want};
-#pragma unroll 1
-        for (uint32_t r = 0; r < w.ranks; r++) { b.lo = min(b.lo, peer_u32(&s.least, r)); b.hi = max(b.hi, peer_u32(&s.most, r)); }
+        const Border b = {__reduce_min_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.least, lane) : 0xFFFFFFFFu),
+                          __reduce_max_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.most, lane) : 0u), (u64)w.listed(), above, want};
         lo = b.lo;
         hi = b.hi;
         if (b.count > 0 && b.count <= kSampleList) {
             cut_in_list<true>(w, b);
         } else if (b.count > kSampleList) {
             cluster_meet();                                      // (everyone has read their number)
-            if (w.rank == 0 && tid == 0) s.list_n = 0;
-            cluster_meet();
+            if (tid == 0) s.list_n = 0;
+            __syncthreads();
             int meetings;
             w.cut = cut_at_border<true>(w, b, meetings);
+            w.whole = false;
         }
     }
     // ---- the choice
@@ -721,20 +818,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const unsigned key = order_of(v[j]);
-            in[j] = key >= lo && key <= hi && w.kept(v[j], i + j) && v[j] >= floor_m;
+            in[j] = key >= lo && key <= hi && (w.whole ? v[j] > -INFINITY : w.kept(v[j], i + j)) && v[j] >= floor_m;
         }
         if (!__any_sync(0xFFFFFFFFu, in[0] || in[1] || in[2] || in[3])) return;
+        u64 wt[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const u64 wt = w.weight(v[j]);
-            if (in[j]) mine += wt;
-        }
+        for (int j = 0; j < 4; j++) wt[j] = w.weight(v[j]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) mine += in[j] ? wt[j] : 0;
     });
-    u64 sum;
-    const u64 run = w.ahead_of_warp(mine, sum);
-    u64 all = 0;
-#pragma unroll 1
-    for (uint32_t r = 0; r < w.ranks; r++) all += peer_u64(&s.answer[0], r);
+    u64 sum, all;
+    const u64 run = w.ahead_of_warp(mine, sum, all);
     cluster_arrive();                                            // nobody leaves before all have read
     const u64 goal = (u64)(u * (double)all) + 1;
     if (run < goal && goal <= run + sum) w.walk(run, goal, share, [&](u64 e) { answer(place_value(e), place_index(e), all); });
