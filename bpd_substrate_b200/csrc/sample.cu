@@ -3,9 +3,10 @@
 // The CTAs of a cluster hold a row between them in shared memory, each a range of the vocabulary, so that it is read once.  A weight
 // w = 2^((x - max) log2(e) / T) is a whole number of 2^-44 (worked out in 64 bits, to 1e-12): sums of 2^18 of them fit 64 bits, are exact, and depend on
 // no order, so neither do the cuts and the choice.  What is kept is always a beginning of the row's order (by value, then by index), hence one
-// place (value, index), the cut.  It is found by a histogram, of numbers over octaves of fp32 weights or of weights over their own leading bits: the bins
-// that certainly lie above are settled, the few elements of the bin that holds the cut are listed in one CTA and compared with each other.  Where
-// those are too many (flat rows, equal values) the bin is halved by exact sums until they are not.
+// place (value, index), the cut.  It is found by a histogram, of numbers over octaves of fp32 weights or of weights over their own leading bits (exact: three
+// numbers of 15 bits a weight, as shared memory adds 32): the bins above are settled, the few elements of the bin that holds the cut are listed in one
+// CTA and compared with each other.  Where those are too many (flat rows, equal values) the bin is halved by exact sums until they are not.  Its own
+// histogram tells a CTA what it holds of the kept weights, so only the one with the chosen token walks through them.
 #include "cluster_device.cuh"
 #include "launch.cuh"
 #include "paged.cuh"
@@ -14,11 +15,12 @@ namespace bpdq {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kCountBins = 2048, kCountOctave = 32;         // numbers: bins, bins per octave of weight
-constexpr int kMassBins = 5888, kMassOctave = 128;          // weights: the 46 octaves down to 2^-45
+constexpr int kMassBins = 1472;                             // weights: 32 per octave for the 46 octaves down to 2^-45
 constexpr int kSampleList = 1024;                           // elements that are sorted
 constexpr int kSampleCounted = 256;                         // elements that are compared with each other instead
 constexpr int kSampleBits = 44;
 constexpr int kSampleMaxVocab = 1 << 18;
+constexpr int kSampleSteps = kSampleMaxVocab / 8 / 128;     // of 128 elements, in a CTA's largest range
 constexpr double kLog2e = 1.4426950408889634074;
 typedef unsigned long long u64;
 
@@ -34,12 +36,13 @@ struct SampleArgs {
 struct SampleShared {
     u64 list[kSampleList];                                  // places
     u64 weight[kSampleList];
-    unsigned hist[kMassBins];
-    double octave[64];
+    ulonglong2 pair[kSampleCounted];                        // place, weight
+    unsigned hist[3 * kMassBins];
+    u64 octave[64], octaves[64], bin[32];
+    u64 step[kSampleSteps];
     u64 red[2][2], warp_red[kSampleWarps][2], warp_sum[kSampleWarps];
     unsigned exp_lo[32], exp_hi[32];
     unsigned list_n, found[4], least, most;
-    float from, to;
     u64 answer[3];
 };
 
@@ -66,7 +69,6 @@ __device__ __forceinline__ unsigned peer_u32(const unsigned* p, uint32_t rank)
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(p, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ double peer_f64(const double* p, uint32_t rank) { return __longlong_as_double((long long)peer_u64(reinterpret_cast<const u64*>(p), rank)); }
 __device__ __forceinline__ void peer_store_u64(u64* p, uint32_t rank, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(p, rank)), "l"(v) : "memory"); }
 __device__ __forceinline__ void cluster_meet() { cluster_arrive(); cluster_wait(); }
 
@@ -200,83 +202,86 @@ struct Sampler {
         meetings++;
     }
 
-    // The histogram's weights are multiples of 2^-15 of their octave's smallest.
-    static __device__ __forceinline__ double unit_of(int octave) { return __hiloint2double((1023 + kSampleBits - 15 - octave) << 20, 0); }
-    // This CTA's sums of the histogram's octaves.
-    template <bool kMass> __device__ __forceinline__ void sum_octaves()
+    static __device__ __forceinline__ u64 share_of(float part, u64 all) { return (u64)fmax(ceil((double)part * (double)all), 1.0); }
+    // Bin of a weight 2^44 2^y: by its exponent and its first five bits; rises as it falls.  (At or beyond kMassBins: it rounds to 0.)
+    static __device__ __forceinline__ int mass_bin(double z) { return ((1023 + kSampleBits) << 5) + 31 - (__double2hiint(z) >> 15); }
+    // What this CTA's histogram holds in a bin.
+    template <bool kMass> __device__ __forceinline__ u64 in_bin(int b, uint32_t r) const
+    {
+        if (!kMass) return peer_u32(&s.hist[b], r);
+        return peer_u32(&s.hist[b], r) + ((u64)peer_u32(&s.hist[kMassBins + b], r) << 15) + ((u64)peer_u32(&s.hist[2 * kMassBins + b], r) << 30);
+    }
+    // The first bin, in the histogram of the cluster, up to which the sum reaches `want`, part of the sum of all or (of numbers) k; -1: none; the sum ahead of it and
+    // what it holds.  All threads; one meeting.
+    template <bool kMass> __device__ __forceinline__ int first_bin(float part, int k, u64& before, u64& holds, u64& want)
     {
         __syncthreads();
-        constexpr int octaves = kMass ? kMassBins / kMassOctave : kCountBins / kCountOctave;
         for (int o = warp; o < 64; o += kSampleWarps) {
-            double v = 0.0;
-            if (o < octaves) {
-                if constexpr (kMass) {
-                    const uint4 h = reinterpret_cast<const uint4*>(s.hist)[o * 32 + lane];
-                    v = (double)warp_total((u64)h.x + h.y + h.z + h.w) * unit_of(o);
-                } else {
-                    v = (double)__reduce_add_sync(0xFFFFFFFFu, s.hist[o * 32 + lane]);
-                }
-            }
+            u64 v = 0;
+            const int i = 32 * o + lane;
+            if (kMass && o < kMassBins / 32) v = warp_total(s.hist[i] + ((u64)s.hist[kMassBins + i] << 15) + ((u64)s.hist[2 * kMassBins + i] << 30));
+            if (!kMass) v = __reduce_add_sync(0xFFFFFFFFu, s.hist[i]);
             if (lane == 0) s.octave[o] = v;
         }
-    }
-    // The histogram of the cluster (a warp, after a meeting): octave by octave, then bin by bin.
-    struct Octaves { double two[2], up, all; };              // of octaves 2 lane and 2 lane + 1; sum up to them; sum of all
-    __device__ __forceinline__ Octaves octaves() const
-    {
-        Octaves o = {{0.0, 0.0}, 0.0, 0.0};
+        cluster_meet();
+        // eight threads per octave, a rank each
+        auto eight = [&](u64 v) {
 #pragma unroll
-        for (int r = 0; r < 8; r++)
-            if (r < (int)ranks) {
-                o.two[0] += peer_f64(&s.octave[2 * lane], r);
-                o.two[1] += peer_f64(&s.octave[2 * lane + 1], r);
+            for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+            return v;
+        };
+        const uint32_t r = tid & 7;
+        const u64 octave_sum = eight(r < ranks ? peer_u64(&s.octave[tid >> 3], r) : 0);
+        if (r == 0) s.octaves[tid >> 3] = octave_sum;
+        __syncthreads();
+        const u64 two0 = s.octaves[2 * lane], two1 = s.octaves[2 * lane + 1], up = warp_scan(two0 + two1, lane);
+        want = (u64)k;
+        if (kMass) want = share_of(part, __shfl_sync(0xFFFFFFFFu, up, 31));
+        const unsigned who0 = __ballot_sync(0xFFFFFFFFu, up - two1 >= want), who1 = __ballot_sync(0xFFFFFFFFu, up >= want);
+        if (!who1) {
+            before = __shfl_sync(0xFFFFFFFFu, up, 31);
+            holds = 0;
+            return -1;
+        }
+        const int l0 = who0 ? __ffs(who0) - 1 : 32, lead = min(l0, __ffs(who1) - 1), octave = 2 * lead + (l0 == lead ? 0 : 1);
+        const u64 ahead = __shfl_sync(0xFFFFFFFFu, up - two1 - (l0 == lead ? two0 : 0), lead);
+        const u64 bin_sum = eight(tid < 256 && r < ranks ? in_bin<kMass>(32 * octave + (tid >> 3), r) : 0);
+        if (tid < 256 && r == 0) s.bin[tid >> 3] = bin_sum;
+        __syncthreads();
+        const u64 mine = s.bin[lane], run = ahead + warp_scan(mine, lane);
+        const int l = __ffs(__ballot_sync(0xFFFFFFFFu, run >= want)) - 1;
+        before = __shfl_sync(0xFFFFFFFFu, run - mine, l);
+        holds = __shfl_sync(0xFFFFFFFFu, mine, l);
+        return 32 * octave + l;
+    }
+    // f(whether it is a kept one of the bin, value, index) for what fp32 does not tell from this CTA's elements of bin b of weights; all lanes together.
+    template <class F> __device__ __forceinline__ void each_in_bin(int bin, F f) const
+    {
+        const int sub = 31 - (bin & 31);
+        // octaves below the largest, and 10^-4 beyond: more than fp32 is off by
+        const float least = (float)(bin >> 5) - log2f(1.0f + (float)(sub + 1) / 32.0f) - 1e-4f, most = (float)(bin >> 5) - log2f(1.0f + (float)sub / 32.0f) + 1e-4f;
+        each([&](const float (&v)[4], int i) {
+            unsigned maybe = 0, sure = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float d = (top - v[j]) * rate;
+                if (d >= least && d <= most && (whole || kept(v[j], i + j))) {
+                    maybe |= 1u << j;
+                    if (d > least + 2e-4f && d < most - 2e-4f) sure |= 1u << j;
+                }
             }
-        o.up = warp_scan(o.two[0] + o.two[1], lane);
-        o.all = __shfl_sync(0xFFFFFFFFu, o.up, 31);
-        return o;
-    }
-    // The first bin b for which reached(sum up to b) holds, or -1; the sum ahead of it, and what it holds.
-    template <bool kMass, class R> __device__ __forceinline__ int first_bin(const Octaves& o, R reached, double& before, double& holds) const
-    {
-        constexpr int n = (kMass ? kMassOctave : kCountOctave) / 32;
-        const unsigned who0 = __ballot_sync(0xFFFFFFFFu, reached(o.up - o.two[1])), who1 = __ballot_sync(0xFFFFFFFFu, reached(o.up));
-        before = o.all;
-        holds = 0.0;
-        if (!(who0 | who1)) return -1;
-        const int l0 = who0 ? __ffs(who0) - 1 : 32, l1 = who1 ? __ffs(who1) - 1 : 32, lead = min(l0, l1), octave = 2 * lead + (l0 <= l1 ? 0 : 1);
-        double run = __shfl_sync(0xFFFFFFFFu, o.up - o.two[1] - (l0 <= l1 ? o.two[0] : 0.0), lead);
-        u64 h[n];
+            if (!__any_sync(0xFFFFFFFFu, maybe)) return;
+            // at the bin's ends the weight itself tells
+            if (__any_sync(0xFFFFFFFFu, maybe != sure)) {
+#pragma unroll 1
+                for (int j = 0; j < 4; j++) {
+                    const float a = j == 0 ? v[0] : (j == 1 ? v[1] : (j == 2 ? v[2] : v[3]));
+                    if (mass_bin(scaled(a)) == bin) sure |= maybe & 1u << j;
+                }
+            }
 #pragma unroll
-        for (int i = 0; i < n; i++) h[i] = 0;
-#pragma unroll
-        for (int r = 0; r < 8; r++)
-            if (r < (int)ranks)
-#pragma unroll
-                for (int i = 0; i < n; i++) h[i] += peer_u32(&s.hist[32 * n * octave + n * lane + i], r);
-        u64 mine = 0;
-#pragma unroll
-        for (int i = 0; i < n; i++) mine += h[i];
-        const double unit = kMass ? unit_of(octave) : 1.0;
-        run += (double)(warp_scan(mine, lane) - mine) * unit;
-        int at = n;
-        double sum = run;
-#pragma unroll
-        for (int i = 0; i < n; i++) {
-            sum += (double)h[i] * unit;
-            if (at == n && reached(sum)) at = i;
-        }
-        const unsigned who = __ballot_sync(0xFFFFFFFFu, at < n);
-        const int l = who ? __ffs(who) - 1 : 31;
-        if (at == n) at = n - 1;            // (sums in another order: the octave's last bin)
-        double mine_before = run, mine_holds = 0.0;
-#pragma unroll
-        for (int i = 0; i < n; i++) {
-            if (i < at) mine_before += (double)h[i] * unit;
-            if (i == at) mine_holds = (double)h[i] * unit;
-        }
-        before = __shfl_sync(0xFFFFFFFFu, mine_before, l);
-        holds = __shfl_sync(0xFFFFFFFFu, mine_holds, l);
-        return 32 * n * octave + n * l + __shfl_sync(0xFFFFFFFFu, at, l);
+            for (int j = 0; j < 4; j++) f((sure >> j & 1u) != 0, v[j], i + j);
+        });
     }
 
     // Puts the place where `yes` holds into this CTA's list, while there is room; list_n counts them all.
@@ -301,18 +306,17 @@ struct Sampler {
             for (unsigned i = 32 * (warp / ranks) + lane; i < count; i += 32 * (kSampleWarps / ranks)) s.list[from + i] = peer_u64(&s.list[i], r);
         __syncthreads();
     }
-    // For listed element tid / parts of n <= kSampleCounted: how many of the others lie ahead of it, and the sum of their s.weight; in all of its threads, of
+    // For element tid / parts of the n <= kSampleCounted in s.pair: how many of the others lie ahead of it, and the sum of their weights; in all of its threads, of
     // which there are `parts`, neighbours.
-    __device__ __forceinline__ void counted(int n, int parts, int& ahead, u64& mass) const
+    __device__ __forceinline__ void counted(int n, int parts, u64 mine, int& ahead, u64& mass) const
     {
-        const int j = tid / parts;
         ahead = 0;
         mass = 0;
-        if (j < n) {
-            const u64 mine = s.list[j];
-#pragma unroll 2
-            for (int i = tid & (parts - 1); i < n; i += parts)
-                if (s.list[i] > mine) { ahead++; mass += s.weight[i]; }
+        if (tid / parts < n) {
+            for (int i = tid & (parts - 1); i < n; i += parts) {
+                const ulonglong2 e = s.pair[i];
+                if (e.x > mine) { ahead++; mass += e.y; }
+            }
         }
         for (int o = parts / 2; o > 0; o >>= 1) {
             ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, o);
@@ -462,15 +466,17 @@ __device__ __forceinline__ void cut_in_list(Sampler& w, const Border& b)
         w.collect();
         auto one = [&](u64 place) -> u64 { return kMass ? w.weight(place_value(place)) : 1; };
         if (n <= kSampleCounted) {
-            if (w.tid < n) s.weight[w.tid] = one(s.list[w.tid]);
+            if (w.tid < n) s.pair[w.tid] = make_ulonglong2(s.list[w.tid], one(s.list[w.tid]));
             __syncthreads();
             const int parts = Sampler::parts_for(n), j = w.tid / parts;
+            ulonglong2 mine = make_ulonglong2(0, 0);
+                if (j < n) mine = s.pair[j];
             int ahead;
             u64 mass;
-            w.counted(n, parts, ahead, mass);
+            w.counted(n, parts, mine.x, ahead, mass);
             // the element that reaches the sum (the last one, should none)
-            if (j < n && b.above + mass < b.want && (b.above + mass + s.weight[j] >= b.want || ahead == n - 1))
-                for (int r = w.tid & (parts - 1); r < (int)w.ranks; r += parts) peer_store_u64(&s.answer[2], (uint32_t)r, s.list[j]);
+            if (j < n && b.above + mass < b.want && (b.above + mass + mine.y >= b.want || ahead == n - 1))
+                for (int r = w.tid & (parts - 1); r < (int)w.ranks; r += parts) peer_store_u64(&s.answer[2], (uint32_t)r, mine.x);
         } else {
             sort_list(s.list, n, w.tid);
             w.scan_weights(n, [&](int i) -> u64 { return one(s.list[i]); });
@@ -479,17 +485,30 @@ __device__ __forceinline__ void cut_in_list(Sampler& w, const Border& b)
         }
     }
     cluster_meet();
-    if (w.tid == 0) w.s.list_n = 0;
     w.cut = w.s.answer[2];
     w.whole = false;
 }
-// Lists the border's elements (list_n is 0), then as above.
+// The same of any number of elements, the kept ones whose bin of the histogram is b (count of them).
 template <bool kMass>
-__device__ __noinline__ u64 cut_at_border(Sampler w, Border b, int& meetings)
+__device__ __noinline__ u64 cut_in_bin(Sampler w, int bin, u64 count, u64 above, u64 want)
 {
-    const bool known = narrow<kMass>(w, b);
-    meetings = w.meetings;
-    if (known) return w.cut;
+    SampleShared& s = w.s;
+    auto in = [&](float v, int i) { return v > -INFINITY && w.kept(v, i) && (kMass ? Sampler::mass_bin(w.scaled(v)) : w.bin_of(v)) == bin; };
+    unsigned lo = 0xFFFFFFFFu, hi = 0;
+    w.each([&](const float (&v)[4], int i) {
+#pragma unroll 1
+        for (int j = 0; j < 4; j++)
+            if (in(v[j], i + j)) { lo = min(lo, order_of(v[j])); hi = max(hi, order_of(v[j])); }
+    });
+    lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+    hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+    if (w.tid == 0) { s.least = 0xFFFFFFFFu; s.most = 0; s.list_n = 0; }
+    __syncthreads();
+    if (w.lane == 0) { atomicMin(&s.least, lo); atomicMax(&s.most, hi); }
+    cluster_meet();
+    Border b = {__reduce_min_sync(0xFFFFFFFFu, w.lane < w.ranks ? peer_u32(&s.least, w.lane) : 0xFFFFFFFFu),
+                __reduce_max_sync(0xFFFFFFFFu, w.lane < w.ranks ? peer_u32(&s.most, w.lane) : 0u), count, above, want};
+    if (narrow<kMass>(w, b)) return w.cut;
     w.each([&](const float (&v)[4], int i) {
 #pragma unroll 1
         for (int j = 0; j < 4; j++) {
@@ -521,8 +540,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
         s.exp_lo[tid] = (unsigned)__double2loint(t);
         s.exp_hi[tid] = (unsigned)__double2hiint(t);
     }
-    if (tid == 0) { s.list_n = 0; s.least = 0xFFFFFFFFu; s.most = 0; }
-    for (int i = tid; i < kMassBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) s.list_n = 0;
+    for (int i = tid; i < 3 * kMassBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
     pdl_wait();
     pdl_launch_dependents();
 
@@ -608,16 +627,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             for (int j = 0; j < 4; j++)
                 if (v[j] > -INFINITY) atomicAdd(&s.hist[w.bin_of(v[j])], 1u);
         });
-        w.sum_octaves<false>();
-        cluster_meet();
-        if (warp == 0) {
-            double before, holds;
-            const int b = w.first_bin<false>(w.octaves(), [&](double up) { return up >= (double)k; }, before, holds);
-            // elements in bins up to it (all, where there are fewer than k)
-            if (lane == 0) { s.found[1] = (unsigned)(b < 0 ? kCountBins : b); s.found[2] = (unsigned)before; s.found[3] = (unsigned)holds; }
-        }
-        __syncthreads();
-        const int b = (int)s.found[1], above = (int)s.found[2], in_bin = (int)s.found[3];
+        u64 before, holds, want;
+        const int found = w.first_bin<false>(0.0f, k, before, holds, want);
+        const int b = found < 0 ? kCountBins : found, above = (int)before, in_bin = (int)holds;      // (all, where there are fewer than k)
         if (above + in_bin <= kSampleList) {
             // ---- few enough for one CTA to finish
             w.each([&](const float (&v)[4], int i) {
@@ -639,32 +651,35 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             if (n <= kSampleCounted) {
                 // An element is kept if fewer than k and less than the share of top_p lie ahead of it: both counted from the list as it is.
                 const int parts = Sampler::parts_for(n), j = tid / parts;
-                if (tid < n) s.weight[tid] = w.weight(place_value(s.list[tid]));
+                if (tid < n) s.pair[tid] = make_ulonglong2(s.list[tid], w.weight(place_value(s.list[tid])));
                 __syncthreads();
-                const u64 mine = j < n ? s.list[j] : 0, wt = j < n ? s.weight[j] : 0;
+                ulonglong2 mine = make_ulonglong2(0, 0);
+                if (j < n) mine = s.pair[j];
                 int ahead;
                 u64 mass;
-                w.counted(n, parts, ahead, mass);
+                w.counted(n, parts, mine.x, ahead, mass);
                 const bool lead = (tid & (parts - 1)) == 0, in_k = j < n && ahead < k;
-                const u64 all_k = w.cta_total(lead && in_k ? wt : 0);
-                const u64 want = cut_p ? (u64)fmax(ceil((double)part * (double)all_k), 1.0) : ~0ull;
-                const bool keep = in_k && mass < want && place_value(mine) >= floor_m;
-                if (lead && j < n) s.weight[j] = keep ? wt : 0;
-                const u64 sum = w.cta_total(lead && keep ? wt : 0), goal = (u64)(u * (double)sum) + 1;
+                const u64 all_k = w.cta_total(lead && in_k ? mine.y : 0);
+                const u64 want = cut_p ? Sampler::share_of(part, all_k) : ~0ull;
+                const bool keep = in_k && mass < want && place_value(mine.x) >= floor_m;
+                if (lead && j < n && !keep) s.pair[j].y = 0;
+                const u64 sum = w.cta_total(lead && keep ? mine.y : 0), goal = (u64)(u * (double)sum) + 1;
                 u64 upto = 0;                                    // of indices up to its own
                 if (keep)
-#pragma unroll 2
-                    for (int i = tid & (parts - 1); i < n; i += parts)
-                        if ((unsigned)s.list[i] >= (unsigned)mine) upto += s.weight[i];
+#pragma unroll 4
+                    for (int i = tid & (parts - 1); i < n; i += parts) {
+                        const ulonglong2 e = s.pair[i];
+                        if ((unsigned)e.x >= (unsigned)mine.x) upto += e.y;
+                    }
                 for (int o = parts / 2; o > 0; o >>= 1) upto += __shfl_xor_sync(0xFFFFFFFFu, upto, o);
-                if (lead && keep && upto >= goal && upto - wt < goal) answer(place_value(mine), place_index(mine), sum);
+                if (lead && keep && upto >= goal && upto - mine.y < goal) answer(place_value(mine.x), place_index(mine.x), sum);
                 return;
             }
             sort_list(s.list, n, tid);
             int keep = n < k ? n : k;
             w.scan_weights(keep, [&](int i) { return w.weight(place_value(s.list[i])); });
             if (cut_p) {
-                const int at = w.first_reaching(keep, (u64)fmax(ceil((double)part * (double)s.weight[keep - 1]), 1.0));
+                const int at = w.first_reaching(keep, Sampler::share_of(part, s.weight[keep - 1]));
                 keep = at < keep ? at + 1 : keep;
             }
             if (cut_m) {
@@ -698,38 +713,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
             return;
         }
         if (b < kCountBins) {
-            // the bin's keys, then its elements
-            unsigned lo = 0xFFFFFFFFu, hi = 0;
-            w.each([&](const float (&v)[4], int) {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (v[j] > -INFINITY && w.bin_of(v[j]) == b) { lo = min(lo, order_of(v[j])); hi = max(hi, order_of(v[j])); }
-            });
-            lo = __reduce_min_sync(0xFFFFFFFFu, lo);
-            hi = __reduce_max_sync(0xFFFFFFFFu, hi);
-            if (lane == 0) { atomicMin(&s.least, lo); atomicMax(&s.most, hi); }
-            cluster_meet();
-            lo = __reduce_min_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.least, lane) : 0xFFFFFFFFu);
-            hi = __reduce_max_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.most, lane) : 0u);
-            int meetings;
-            w.cut = cut_at_border<false>(w, Border{lo, hi, (u64)in_bin, (u64)above, (u64)k}, meetings);
-            w.meetings = meetings;
+            w.cut = cut_in_bin<false>(w, b, (u64)in_bin, (u64)above, (u64)k);
             w.whole = false;
         }
         if (cut_p) {
-            cluster_meet();                                      // (the histogram and the bounds are still being read)
-            for (int i = tid; i < kMassBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
-            if (tid == 0) { s.least = 0xFFFFFFFFu; s.most = 0; }
+            cluster_meet();                                      // (the histogram is still being read)
+            for (int i = tid; i < 3 * kMassBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
+            if (tid == 0) s.list_n = 0;
             __syncthreads();
         }
     }
-    // what the choice is made by, as far as it is known: places above the bins with the cut
+    // ---- what this CTA holds of the kept weights
     u64 mine = 0;
-    unsigned lo = 0, hi = 0xFFFFFFFFu;                           // keys of elements that are not in it yet
     if (cut_p) {
-        u64 sum = 0, nothing = 0;
-        // per bin, of the weights' leading bits, what they begin with in multiples of 2^-15, rounded up: within 2^-14 of the bin's sum
-        constexpr int first_key = ((1023 + kSampleBits) << 7) + 127;
         w.each([&](const float (&v)[4], int i) {
             double z[4];
 #pragma unroll
@@ -737,101 +733,123 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (!w.whole && !w.kept(v[j], i + j)) z[j] = 0.0;
-                sum += Sampler::whole_of(z[j]);
-                const int hi = __double2hiint(z[j]), b = first_key - (hi >> 13);
-                if (b < kMassBins) atomicAdd(&s.hist[b], ((unsigned)((hi & 0xFFFFF) | 0x100000) >> 5) + 1u);
+                const int b = Sampler::mass_bin(z[j]);
+                const u64 wt = Sampler::whole_of(z[j]);
+                if (b < kMassBins) {
+                    atomicAdd(&s.hist[b], (unsigned)wt & 0x7FFFu);
+                    const unsigned middle = (unsigned)(wt >> 15) & 0x7FFFu, upper = (unsigned)(wt >> 30);
+                    if (middle) atomicAdd(&s.hist[kMassBins + b], middle);
+                    if (upper) atomicAdd(&s.hist[2 * kMassBins + b], upper);
+                }
             }
         });
-        w.sum_octaves<true>();
-        w.total(sum, nothing);
-        const u64 want = (u64)fmax(ceil((double)part * (double)sum), 1.0);
-        if (warp == 0) {
-            // the sum up to a bin from either side: whichever is less is known better
-            const double m = (double)sum, goal = (double)want, slack = (double)p.vocab, err = 1.0 / 16384.0;
-            const typename Sampler::Octaves o = w.octaves();
-            double before, holds;
-            const int b1 = w.first_bin<true>(o, [&](double up) { return fmin(up * (1.0 + err), m - fmax(o.all - up, 0.0) * (1.0 - err)) + slack >= goal; }, before, holds);
-            const int b2 = w.first_bin<true>(o, [&](double up) { return fmax(up * (1.0 - err), m - fmax(o.all - up, 0.0) * (1.0 + err)) - slack >= goal; }, before, holds);
-            // the logits at the ends of bins b1 .. b2, and 1e-13 octaves beyond, which weights are not off by
-            if (lane < 2) {
-                const int bin = lane == 0 ? b1 : b2, key = first_key - bin + (lane == 0 ? 1 : 0);
-                const double at = w.top64 + (log2(__hiloint2double(key << 13, 0)) - (double)kSampleBits + (lane == 0 ? 1e-13 : -1e-13)) / w.rate64;
-                if (lane == 0) s.to = bin < 0 ? -INFINITY : __double2float_ru(at);
-                else s.from = bin < 0 ? -INFINITY : __double2float_rd(at);
+        bool in_list = false;                                    // the elements of the cut's bin are this CTA's list
+        u64 above, holds, want;
+        const int b = w.first_bin<true>(part, 0, above, holds, want);
+        if (b >= 0) {
+            w.each_in_bin(b, [&](bool yes, float v, int i) { w.list_if(yes, place_of(v, i)); });
+            cluster_meet();
+            const u64 count = w.listed();
+            if (count <= kSampleList) {
+                Border border;
+                border.lo = border.hi = 0;
+                border.count = count;
+                border.above = above;
+                border.want = want;
+                cut_in_list<true>(w, border);
+                in_list = w.rank != 0 || count <= kSampleCounted;        // (longer ones have been sorted there, with the others')
+            } else {
+                cluster_meet();                                  // (everyone has read the number)
+                w.cut = cut_in_bin<true>(w, b, count, above, want);
+                w.whole = false;
             }
         }
-        __syncthreads();
-        const float from = s.from, to = s.to;
-        // the exact sum above, and the elements of the bins with the cut
-        u64 above = 0;
-        lo = 0xFFFFFFFFu;
-        hi = 0;
+        const u64 floor_place = (u64)order_of(floor_m) << 32;
+        if (floor_m > -INFINITY && floor_place > w.cut) { w.cut = floor_place; w.whole = in_list = false; }
+        // the bins above the cut's, by the CTA's own histogram, and of that bin the elements from the cut on
+        int last = kMassBins;
+        if (!w.whole) {
+            const int of_cut = Sampler::mass_bin(w.scaled(place_value(w.cut)));
+            if (of_cut < last) last = of_cut;
+        }
+        for (int i = tid; i < last; i += kSampleThreads) mine += s.hist[i] + ((u64)s.hist[kMassBins + i] << 15) + ((u64)s.hist[2 * kMassBins + i] << 30);
+        if (in_list) {
+            const int own = (int)s.list_n;
+            for (int i = tid; i < own; i += kSampleThreads)
+                if (s.list[i] >= w.cut) mine += w.weight(place_value(s.list[i]));
+        } else if (last < kMassBins) w.each_in_bin(last, [&](bool yes, float v, int) { if (yes) mine += w.weight(v); });
+    } else {
+        const u64 floor_place = (u64)order_of(floor_m) << 32;
+        if (floor_m > -INFINITY && floor_place > w.cut) { w.cut = floor_place; w.whole = false; }
         w.each([&](const float (&v)[4], int i) {
-            bool over[4], in[4];
+            bool in[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool yes = v[j] > -INFINITY && (w.whole || w.kept(v[j], i + j));
-                over[j] = yes && v[j] > to;
-                in[j] = yes && v[j] <= to && v[j] >= from;
-            }
-            if (__any_sync(0xFFFFFFFFu, over[0] || over[1] || over[2] || over[3])) {
-                u64 wt[4];
+            for (int j = 0; j < 4; j++) in[j] = w.whole || w.kept(v[j], i + j);
+            if (!__any_sync(0xFFFFFFFFu, in[0] || in[1] || in[2] || in[3])) return;
+            u64 wt[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) wt[j] = w.weight(v[j]);
+            for (int j = 0; j < 4; j++) wt[j] = w.weight(v[j]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    above += over[j] ? wt[j] : 0;
-                    mine += over[j] && v[j] >= floor_m ? wt[j] : 0;
-                }
-            }
-            if (__any_sync(0xFFFFFFFFu, in[0] || in[1] || in[2] || in[3])) {
-#pragma unroll 1
-                for (int j = 0; j < 4; j++) {
-                    if (in[j]) { lo = min(lo, order_of(v[j])); hi = max(hi, order_of(v[j])); }
-                    w.list_if(in[j], place_of(v[j], i + j));
-                }
-            }
+            for (int j = 0; j < 4; j++) mine += in[j] ? wt[j] : 0;
         });
-        lo = __reduce_min_sync(0xFFFFFFFFu, lo);
-        hi = __reduce_max_sync(0xFFFFFFFFu, hi);
-        if (lane == 0) { atomicMin(&s.least, lo); atomicMax(&s.most, hi); }
-        w.total(above, nothing);
-        const Border b = {__reduce_min_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.least, lane) : 0xFFFFFFFFu),
-                          __reduce_max_sync(0xFFFFFFFFu, lane < w.ranks ? peer_u32(&s.most, lane) : 0u), (u64)w.listed(), above, want};
-        lo = b.lo;
-        hi = b.hi;
-        if (b.count > 0 && b.count <= kSampleList) {
-            cut_in_list<true>(w, b);
-        } else if (b.count > kSampleList) {
-            cluster_meet();                                      // (everyone has read their number)
-            if (tid == 0) s.list_n = 0;
-            __syncthreads();
-            int meetings;
-            w.cut = cut_at_border<true>(w, b, meetings);
-            w.whole = false;
-        }
     }
-    // ---- the choice
-    auto share = [&](float v, int i) -> u64 { return w.kept(v, i) && v >= floor_m ? w.weight(v) : 0; };
-    w.each([&](const float (&v)[4], int i) {
-        bool in[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const unsigned key = order_of(v[j]);
-            in[j] = key >= lo && key <= hi && (w.whole ? v[j] > -INFINITY : w.kept(v[j], i + j)) && v[j] >= floor_m;
-        }
-        if (!__any_sync(0xFFFFFFFFu, in[0] || in[1] || in[2] || in[3])) return;
-        u64 wt[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) wt[j] = w.weight(v[j]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) mine += in[j] ? wt[j] : 0;
-    });
-    u64 sum, all;
-    const u64 run = w.ahead_of_warp(mine, sum, all);
+    // ---- the choice: the CTA, then the step of 128 elements, then the element
+    const u64 held = w.cta_total(mine);
+    if (tid == 0) s.answer[0] = held;
+    cluster_meet();
+    const u64 peer = lane < w.ranks ? peer_u64(&s.answer[0], lane) : 0, all = warp_total(peer);
+    u64 run = warp_total(lane < w.rank ? peer : 0);
     cluster_arrive();                                            // nobody leaves before all have read
     const u64 goal = (u64)(u * (double)all) + 1;
-    if (run < goal && goal <= run + sum) w.walk(run, goal, share, [&](u64 e) { answer(place_value(e), place_index(e), all); });
+    if (run < goal && goal <= run + held) {
+        auto share = [&](const float (&v)[4], int i, u64 (&wt)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) wt[j] = w.weight(v[j]);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (!w.whole && !w.kept(v[j], i + j)) wt[j] = 0;
+        };
+        int at = warp * (w.chunk / 128);
+        w.each([&](const float (&v)[4], int i) {
+            u64 wt[4];
+            share(v, i, wt);
+            const u64 sum = warp_total(wt[0] + wt[1] + wt[2] + wt[3]);
+            if (lane == 0) s.step[at] = sum;
+            at++;
+        });
+        __syncthreads();
+        if (warp == 0) {
+            const int steps = kSampleWarps * w.chunk / 128;
+            for (int i0 = 0; i0 < steps; i0 += 32) {
+                const u64 up = run + warp_scan(i0 + lane < steps ? s.step[i0 + lane] : 0, lane);
+                const unsigned who = __ballot_sync(0xFFFFFFFFu, up >= goal);
+                if (!who) {
+                    run = __shfl_sync(0xFFFFFFFFu, up, 31);
+                    continue;
+                }
+                const int l = __ffs(who) - 1, i = 128 * (i0 + l) + 4 * lane;
+                if (l > 0) run = __shfl_sync(0xFFFFFFFFu, up, l - 1);
+                const float4 f = *reinterpret_cast<const float4*>(x + i);
+                const float v[4] = {f.x, f.y, f.z, f.w};
+                u64 wt[4];
+                share(v, w.base + i, wt);
+                u64 sum = run + warp_scan(wt[0] + wt[1] + wt[2] + wt[3], lane);
+                const unsigned in = __ballot_sync(0xFFFFFFFFu, sum >= goal);
+                if (lane == __ffs(in) - 1) {
+                    // its last element at which the sum is still there without those behind it
+                    float value = v[3];
+                    int index = w.base + i + 3;
+#pragma unroll
+                    for (int j = 3; j > 0; j--) {
+                        sum -= wt[j];
+                        if (sum >= goal) { value = v[j - 1]; index = w.base + i + j - 1; }
+                    }
+                    answer(value, index, all);
+                }
+                break;
+            }
+        }
+    }
     cluster_wait();
 }
 
