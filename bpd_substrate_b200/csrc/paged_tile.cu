@@ -1,12 +1,14 @@
 // Attention over a paged cache for jobs of many rows (paged_attention.cuh), on tcgen05: portions of prompts, and prefixes that many sequences share.
 //
 // An item is up to 256 rows of a key head (two tiles of 128, whole tokens each; row = (token, query head)) against blocks of 128 keys; CTAs take equal runs
-// of blocks of all items.  Two streams of work alternate on the tensor pipe, so that one's products run under the other's softmax: the item's two tiles, or, of an
-// item with one, its even and odd blocks, whose sums meet at the end.
-//   warp 0      tiled bulk copies of queries, and of keys and values page by page, into 128-byte-swizzled shared memory
-//   warp 1      tensor memory, MMAs: after a step's O += P V its stream's next scores S = Q K^T
+// of blocks of all items.  Two streams of work share the tensor pipe: the item's two tiles, or, of an item with one, the halves of every block, whose sums meet at the
+// end.  A step is 64 keys; a stream has two sets of scores, so that products run under the softmax of the step before.
+//   warps 0, 2  tiled bulk copies of queries and keys, and of values, page by page, into 128-byte-swizzled shared memory
+//   warps 1, 3  tensor memory, MMAs of a stream each: after a step's O += P V the scores S = Q K^T of the step after next
 //   warps 4-11  softmax, four per stream, a thread per row; weights go back to tensor memory over the scores they came from.  (The tensor pipe works
 //               its products off in the order in which they are issued: scores do not overtake the product that reads the weights beneath them.)
+// (Every barrier of a stream's steps comes twice, for even and odd ones: a role may be two steps ahead of another.)
+// The streams take their exponentials in turns: both at once would wait for the special function unit together and leave it idle together.
 // O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8 since the last time.  Weights are rounded to the cache's type: half
 // a step (2^-9 of a bf16 weight on average) of each, which the sum over keys averages to below the result's own rounding.  fp32 activations bring queries and weights as two
 // fp16 numbers each: four products where 16 bits take two, and one tile per item.
@@ -18,7 +20,7 @@
 
 namespace bpdq {
 
-constexpr int kPtRows = 128, kPtKeys = 128, kPtPiece = 128 * 64 * 2;        // rows of a tile, keys of a block, bytes of 128 rows x 64 columns
+constexpr int kPtRows = 128, kPtKeys = 128, kPtStep = 64, kPtPiece = 128 * 64 * 2;     // rows of a tile, keys of a block and of a step, bytes of 128 rows x 64 columns
 constexpr int kPtWarps = 8, kPtThreads = 32 * (4 + kPtWarps);          // three groups of four warps, which have registers of their own size
 constexpr float kPtGrowth = 8.0f;
 
@@ -54,6 +56,37 @@ __device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint
     lo = pack_16<__half>(v0 - f.x, v1 - f.y);
 }
 
+// Two fp32 numbers at once.
+__device__ __forceinline__ float2 fma_two(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add_two(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 2^x of two numbers without the special function unit: x = n + f, |f| <= 1/2, and a polynomial of degree 4 (fitted over that range, off by 3e-6: a weight
+// keeps 8 to 11 bits).  0 from 2^-127 down.
+__device__ __forceinline__ float2 ex2_two(float2 x)
+{
+    x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
+    const float2 shift = make_float2(12582912.0f, 12582912.0f), back = make_float2(-12582912.0f, -12582912.0f), minus = make_float2(-1.0f, -1.0f);
+    const float2 k = add_two(x, shift), f = fma_two(add_two(k, back), minus, x);
+    float2 p = make_float2(9.5605102e-3f, 9.5605102e-3f);
+    p = fma_two(p, f, make_float2(5.5917039e-2f, 5.5917039e-2f));
+    p = fma_two(p, f, make_float2(2.4024981e-1f, 2.4024981e-1f));
+    p = fma_two(p, f, make_float2(6.9312197e-1f, 6.9312197e-1f));
+    p = fma_two(p, f, make_float2(9.9999919e-1f, 9.9999919e-1f));
+    const float2 n = make_float2(__int_as_float((__float_as_int(k.x) << 23) + 0x3F800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3F800000));
+    return fma_two(p, n, make_float2(0.0f, 0.0f));
+}
 // An item: a key head's rows of some tokens of a job.
 struct PtItem {
     PagedJob job;
@@ -70,7 +103,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     constexpr bool f32 = sizeof(A) == 4;
     constexpr int kHalves = Shape::halves, kDepth = Shape::depth;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t q_full, q_empty, k_full[kDepth], k_empty[kDepth], v_full[kDepth], v_empty[kDepth], s_full[2], p_full[2], o_done[2], ml_ready, o1_free;
+    __shared__ uint64_t q_full, q_empty, k_full[kDepth], k_empty[kDepth], v_full[kDepth], v_empty[kDepth], s_full[2][2], p_full[2][2], o_done[2][2], ml_ready, o1_free, turn[2];
     __shared__ uint32_t tmem_slot;
     __shared__ unsigned short s_missing[8];             // of a block: groups of eight keys without a page; softmax is two blocks behind the copies' kDepth at most
     __shared__ float2 s_ml[kPtRows];
@@ -78,13 +111,19 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     uint8_t* base = raw + (((smem_addr(raw) + 1023) & ~1023u) - smem_addr(raw));
     uint8_t *sq = base + Shape::q, *sk = base + Shape::k, *sv = base + Shape::v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+        if (!f32) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
+    }
     if (tid == 0) {
         mbar_init(&q_full, f32 ? kPtWarps : 1);
-        mbar_init(&q_empty, 1);
-        for (int i = 0; i < kDepth; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+        mbar_init(&q_empty, 2);
+        for (int i = 0; i < kDepth; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 2); }
+        for (int i = 0; i < 2; i++) { mbar_init(&s_full[0][i], 1); mbar_init(&s_full[1][i], 1); mbar_init(&p_full[0][i], 4); mbar_init(&p_full[1][i], 4); mbar_init(&o_done[0][i], 1); mbar_init(&o_done[1][i], 1); }
         mbar_init(&ml_ready, 4);
         mbar_init(&o1_free, 4);
+        mbar_init(&turn[0], 4); mbar_init(&turn[1], 4);
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -93,8 +132,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (warp >= 8 && lane == 0) mbar_arrive(&turn[0]);          // the first stream begins
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_slot;                    // scores of stream s in columns 128 s on, its sums in columns 256 + 128 s on
+    const uint32_t tmem = tmem_slot;                    // scores of stream s in columns 128 s and 128 s + 64 on, its sums in columns 256 + 128 s on
     pdl_wait();
     pdl_launch_dependents();
 
@@ -136,7 +176,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         it.from = it.job.from + at * kPtKeys;
         it.blocks = min(it.end, u1) - u;
     };
-    // two tiles, each against every block; or one, its blocks in turn
+    // Two tiles, each against every block, step t against half t % 2 of block t / 2; or one, stream s against half s of block t.
     auto is_dual = [&](const PtItem& it) { return !f32 && it.tokens > tile_tokens; };
 
     // of 168 registers a thread at launch: 4 * 56 + 8 * 224 = 12 * 168
@@ -144,7 +184,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ---------------- softmax
         const int s = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
-        const uint32_t lanes = (uint32_t)(32 * quarter) << 16, ts = tmem + lanes + 128 * s, to_ = tmem + lanes + 256;
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16, to_ = tmem + lanes + 256;
         PtItem it = {};
         int nk = 0, steps = 0, items = 0, meets = 0;
         bool ok = true;
@@ -194,43 +234,46 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             const float sign = f < 0.0f ? -1.0f : 1.0f;
             f = fabsf(f);
             float top = -INFINITY, sum = 0.0f;          // in units of log2
-            int n = s;
-            for (; n < n_steps; n += 2, steps++) {
-                const int b = dual ? n >> 1 : n, key = it.from + b * kPtKeys;
-                if (!mbar_wait_bounded(&s_full[s], (uint32_t)steps & 1u, err, 92)) { ok = false; break; }
+            for (int t = 0; t < n_steps; t++, steps++) {
+                const int b = dual ? t >> 1 : t, half = dual ? t & 1 : s, key = it.from + b * kPtKeys + half * kPtStep;
+                const uint32_t ts = tmem + lanes + 128 * s + 64 * (steps & 1);
+                if (!mbar_wait_bounded(&s_full[s][steps & 1], (uint32_t)(steps >> 1) & 1u, err, 92)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                float v[128];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld_32(ts + 32 * c, v + 32 * c);
+                float v[64];
+                tmem_ld_32(ts, v);
+                tmem_ld_32(ts + 32, v + 32);
                 tmem_loaded();
-                const unsigned missing = s_missing[(nk + b) & 7];
-                const bool edge = __any_sync(0xFFFFFFFFu, key + kPtKeys > limit || missing);
+                const unsigned missing = s_missing[(nk + b) & 7] >> (8 * half) & 0xFFu;
+                const bool edge = __any_sync(0xFFFFFFFFu, key + kPtStep > limit || missing);
                 float ff = f;
                 if (p.cap > 0.0f) {
                     const float in = sign * f * 0.69314718055994531f;
 #pragma unroll
-                    for (int j = 0; j < 128; j++) v[j] = capped<f32>(v[j] * in, p.cap) * 1.44269504088896341f;
+                    for (int j = 0; j < 64; j++) v[j] = capped<f32>(v[j] * in, p.cap) * 1.44269504088896341f;
                     ff = 1.0f;
                 } else if (sign < 0.0f) {
 #pragma unroll
-                    for (int j = 0; j < 128; j++) v[j] = -v[j];
+                    for (int j = 0; j < 64; j++) v[j] = -v[j];
                 }
                 if (edge) {
 #pragma unroll
-                    for (int j = 0; j < 128; j++) v[j] = key + j < limit && !(missing >> (j >> 3) & 1u) ? v[j] * ff : -INFINITY;
+                    for (int j = 0; j < 64; j++) v[j] = key + j < limit && !(missing >> (j >> 3) & 1u) ? v[j] * ff : -INFINITY;
                     ff = 1.0f;
                 }
                 float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int j = 4; j < 128; j++) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+                for (int j = 4; j < 64; j += 8) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) m4[i] = j + 4 < 64 ? fmaxf(fmaxf(m4[i], v[j + i]), v[(j + 4 + i) & 63]) : fmaxf(m4[i], v[j + i]);
+                }
                 const float now = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * ff;
                 const bool grown = now > top + kPtGrowth;
-                if (n > 1 && __any_sync(0xFFFFFFFFu, grown)) {
-                    if (!mbar_wait_bounded(&o_done[s], (uint32_t)(steps - 1) & 1u, err, 93)) { ok = false; break; }
+                if (t > 0 && __any_sync(0xFFFFFFFFu, grown)) {
+                    if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 93)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const float down = grown ? ex2(top - now) : 1.0f;
                     sum *= down;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
                         int ov[16];
                         tmem_ld(to_ + 128 * s + c, ov);
@@ -243,50 +286,59 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 }
                 if (grown) top = now;
                 const float zero = top == -INFINITY ? 0.0f : top;
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (!mbar_wait_bounded(&turn[s], (uint32_t)steps & 1u, err, 98)) { ok = false; break; }
+                const float2 f2 = make_float2(ff, ff), zero2 = make_float2(-zero, -zero);
+                float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
 #pragma unroll
-                    for (int j = 32 * c; j < 32 * c + 32; j++) {
-                        v[j] = ex2(fmaf(v[j], ff, -zero));
-                        part[j & 3] += v[j];
+                    for (int j = 32 * c; j < 32 * c + 32; j += 2) {
+                        float2 x = fma_two(make_float2(v[j], v[j + 1]), f2, zero2);
+                        if (!f32 && (j & 6) == 6) {
+                            x = ex2_two(x);             // every fourth pair, on pipes that the others leave idle
+                        } else {
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
+                        }
+                        part[(j >> 1) & 1] = add_two(part[(j >> 1) & 1], x);
+                        v[j] = x.x;
+                        v[j + 1] = x.y;
                     }
                     uint32_t hi[16];
                     if constexpr (f32) {
                         uint32_t lo[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) split_f16(v[32 * c + 2 * j], v[32 * c + 2 * j + 1], hi[j], lo[j]);
-                        tmem_st(ts + 64 + 16 * c, lo);
+                        tmem_st(ts + 32 + 16 * c, lo);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 16; j++) hi[j] = pack_16<K>(v[32 * c + 2 * j], v[32 * c + 2 * j + 1]);
                     }
                     tmem_st(ts + 16 * c, hi);
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                if (key + kPtKeys > it.job.to || missing) {
-                    // whatever lies in places that hold no position must not meet a weight, not even one of 0: a thread per key
-                    const int slot = (nk + b) % kDepth;
+                if (lane == 0) mbar_arrive(&turn[1 - s]);
+                sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                if (key + kPtStep > it.job.to || missing) {
+                    // whatever lies in places that hold no position must not meet a weight, not even one of 0: two threads per key
+                    const int slot = (nk + b) % kDepth, mine = r >> 1;
                     if (!mbar_wait_bounded(&v_full[slot], (uint32_t)((nk + b) / kDepth) & 1u, err, 94)) { ok = false; break; }
-                    if (key + r >= it.job.to || (missing >> (r >> 3) & 1u))
+                    if (key + mine >= it.job.to || (missing >> (mine >> 3) & 1u))
 #pragma unroll
-                        for (int c = 0; c < kHalves * 8; c++)
-                            *reinterpret_cast<uint4*>(sv + (slot * kHalves + (c >> 3)) * kPtPiece + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        for (int c = 0; c < kHalves * 4; c++)
+                            *reinterpret_cast<uint4*>(sv + (slot * kHalves + (c >> 2)) * kPtPiece + (half * kPtStep + mine) * 128 + ((c & 3) * 2 + (r & 1)) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 tmem_stored();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[s]);
+                if (lane == 0) mbar_arrive(&p_full[s][steps & 1]);
             }
             if (!ok) break;
             nk += it.blocks;
             // ---- the item's sums, or this CTA's part of them
-            const bool any = n_steps > s;               // (a single block has no odd ones)
-            if (any && !mbar_wait_bounded(&o_done[s], (uint32_t)(steps - 1) & 1u, err, 95)) { ok = false; break; }
+            if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 95)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float w0 = 1.0f, w1 = 0.0f;
-            const bool both = !dual && n_steps > 1;
             if (!dual) {
                 if (s == 1) s_ml[r] = make_float2(top, sum);
                 __syncwarp();
@@ -300,7 +352,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 if (!mbar_wait_bounded(&ml_ready, (uint32_t)meets & 1u, err, 97)) { ok = false; break; }
                 meets++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (both) {
+                {
                     const float2 odd = s_ml[r];
                     const float most = fmaxf(top, odd.x), zero = most == -INFINITY ? 0.0f : most;
                     w0 = ex2(top - zero);
@@ -321,35 +373,37 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 w0 *= inv;
                 w1 *= inv;
             }
-#pragma unroll
-            for (int c = 0; c < DP; c += 16) {
-                int ov[16];
-                float x[16];
-                tmem_ld(to_ + 128 * s + c, ov);
-                tmem_loaded();
-#pragma unroll
-                for (int j = 0; j < 16; j++) x[j] = __int_as_float(ov[j]) * w0;
-                if (both) {
-                    tmem_ld(to_ + 128 + c, ov);
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                float x[32];
+                tmem_ld_32(to_ + 128 * s + c, x);
+                if (!dual) {
+                    float y[32];
+                    tmem_ld_32(to_ + 128 + c, y);
                     tmem_loaded();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) x[j] = fmaf(__int_as_float(ov[j]), w1, x[j]);
-                }
-                if (!live) continue;
-                if (!direct) {
+                    for (int j = 0; j < 32; j++) x[j] = fmaf(y[j], w1, x[j] * w0);
+                } else {
+                    tmem_loaded();
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(dst + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                    for (int j = 0; j < 32; j++) x[j] *= w0;
+                }
+                if (!live) {
+                } else if (!direct) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(dst + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
                 } else if constexpr (f32) {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4)
+                    for (int j = 0; j < 32; j += 4)
                         if (c + j < p.dim) *reinterpret_cast<float4*>(o + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 8)
+                    for (int j = 0; j < 32; j += 8)
                         if (c + j < p.dim)
                             *reinterpret_cast<uint4*>(o + c + j) = make_uint4(pack_16<K>(x[j], x[j + 1]), pack_16<K>(x[j + 2], x[j + 3]), pack_16<K>(x[j + 4], x[j + 5]),
                                                                               pack_16<K>(x[j + 6], x[j + 7]));
                 }
+                __syncwarp();
             }
             if (live) {
                 if (!direct) (!all ? p.tile_ml : (it.job.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top, sum);
@@ -364,112 +418,132 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0) {
-        // ---------------- copies
-        PtItem it = {};
-        int nk = 0, items = 0;
-        bool ok = true;
-        for (int u = u0; ok && u < u1; u += it.blocks, items++) {
-            open(it, u, u != u0);
-            const bool dual = is_dual(it);
-            if (!f32) {
-                if (items && !mbar_wait_bounded(&q_empty, (uint32_t)(items - 1) & 1u, err, 84)) break;
-                if (lane == 0) {
-                    mbar_expect_tx(&q_full, (uint32_t)((dual ? 2 : 1) * kHalves * tile_tokens * p.share * 128));
-                    for (int s = 0; s < (dual ? 2 : 1); s++)
-#pragma unroll
-                        for (int h = 0; h < kHalves; h++) tma_rows_3d(sq + (s * kHalves + h) * kPtPiece, &qmap, 64 * h, it.head * p.share, it.job.first + it.t0 + s * tile_tokens, &q_full);
-                }
-            }
-            // a lane per page (box) of a block
-            const int box_rows = p.page < kPtKeys ? p.page : kPtKeys, boxes = kPtKeys / box_rows;
-            const int* table = p.table + (size_t)it.job.seq * p.max_pages;
-            auto entry_of = [&](int b) {
-                const int key = it.from + b * kPtKeys + lane * box_rows;
-                return lane < boxes && key < it.job.to ? table[key >> p.log_page] : -2;
-            };
-            int entry = entry_of(0);
-            for (int b = 0; b < it.blocks; b++, nk++) {
-                const int slot = nk % kDepth, now = entry;
-                if (b + 1 < it.blocks) entry = entry_of(b + 1);
-                const bool have = now >= 0 && now < p.n_pages;
-                if (now != -2 && !have) report(err, 82);
-                const unsigned who = __ballot_sync(0xFFFFFFFFu, have);
-                const uint32_t bytes = (uint32_t)(__popc(who) * box_rows * 128 * kHalves);
-                if (nk >= kDepth && !mbar_wait_bounded(&k_empty[slot], (uint32_t)(nk / kDepth - 1) & 1u, err, 85)) { ok = false; break; }
-                if (lane == 0) {
-                    unsigned missing = 0;
-                    for (int g = 0; g < 16; g++)
-                        if (!(who >> (g * 8 / box_rows) & 1u)) missing |= 1u << g;
-                    s_missing[nk & 7] = (unsigned short)missing;
-                    mbar_expect_tx(&k_full[slot], bytes);
-                }
-                __syncwarp();
-                const int row = (it.from + b * kPtKeys + lane * box_rows) & (p.page - 1);
-                if (have)
-                    for (int h = 0; h < (p.both ? 1 : kHalves); h++)
-                        tma_page(smem_addr(sk + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), &kmap, 64 * h, row, it.head, now, smem_addr(&k_full[slot]));
-                if (nk >= kDepth && !mbar_wait_bounded(&v_empty[slot], (uint32_t)(nk / kDepth - 1) & 1u, err, 86)) { ok = false; break; }
-                if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
-                __syncwarp();
-                if (have)
-                    for (int h = 0; h < (p.both ? 1 : kHalves); h++)
-                        tma_page(smem_addr(sv + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), &vmap, 64 * h, row, it.head, now, smem_addr(&v_full[slot]));
-            }
-        }
-        } else if (warp == 1) {
-        // ---------------- MMAs
-        if (elect_one()) {
-            constexpr uint32_t kind = sizeof(K) == 2 && std::is_same<K, bf16>::value ? 1u : 0u;
-            constexpr uint32_t fmt = (1u << 4) | (kind << 7) | (kind << 10) | ((uint32_t)(kPtRows >> 4) << 24);
-            constexpr uint32_t idesc_s = fmt | ((uint32_t)(kPtKeys >> 3) << 17), idesc_o = fmt | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
+        if (warp == 0 || warp == 2) {
+            // ---------------- copies: queries and keys, or values.  (Scores run ahead of sums, so neither may wait for the other's room.)
+            const bool keys = warp == 0;
+            const CUtensorMap* map = keys ? &kmap : &vmap;
+            uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+            uint8_t* room = keys ? sk : sv;
             PtItem it = {};
-            int nk = 0, items = 0, steps[2] = {0, 0};
+            int nk = 0, items = 0;
             bool ok = true;
             for (int u = u0; ok && u < u1; u += it.blocks, items++) {
                 open(it, u, u != u0);
-                const bool dual = is_dual(it);
-                const int n_steps = dual ? 2 * it.blocks : it.blocks;
-                auto block_of = [&](int n) { return dual ? n >> 1 : n; };
-                if (!(ok = mbar_wait_bounded(&q_full, (uint32_t)items & 1u, err, 87))) break;
-                auto scores = [&](int n) {
-                    const int s = n & 1, at = nk + block_of(n), slot = at % kDepth;
-                    if (!mbar_wait_bounded(&k_full[slot], (uint32_t)(at / kDepth) & 1u, err, 88)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t qd = swizzled_desc(smem_addr(sq + (dual ? s : 0) * kHalves * kPtPiece)), kd = swizzled_desc(smem_addr(sk + slot * kHalves * kPtPiece));
+                if (!f32 && keys) {
+                    const int tiles = is_dual(it) ? 2 : 1;
+                    if (items && !mbar_wait_bounded(&q_empty, (uint32_t)(items - 1) & 1u, err, 84)) break;
+                    if (lane == 0) {
+                        mbar_expect_tx(&q_full, (uint32_t)(tiles * kHalves * tile_tokens * p.share * 128));
+                        for (int s = 0; s < tiles; s++)
 #pragma unroll
-                    for (int part = 0; part < (f32 ? 2 : 1); part++)
-#pragma unroll
-                        for (int h = 0; h < kHalves; h++)
-#pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                umma_bf16_ss(tmem + 128 * s, qd + (uint64_t)((part * kHalves + h) * (kPtPiece >> 4) + 2 * k), kd + (uint64_t)(h * (kPtPiece >> 4) + 2 * k), idesc_s,
-                                             part | h | k ? 1u : 0u);
-                    umma_commit(&s_full[s]);
-                    if (!dual || s == 1) umma_commit(&k_empty[slot]);
-                    if (n == n_steps - 1) umma_commit(&q_empty);
-                    return true;
-                };
-                ok = scores(0) && (n_steps < 2 || scores(1));
-                for (int n = 0; ok && n < n_steps; n++) {
-                    const int s = n & 1, at = nk + block_of(n), slot = at % kDepth;
-                    if (!(ok = mbar_wait_bounded(&v_full[slot], (uint32_t)(at / kDepth) & 1u, err, 89) && mbar_wait_bounded(&p_full[s], (uint32_t)steps[s] & 1u, err, 90))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t vd = swizzled_desc_mn(smem_addr(sv + slot * kHalves * kPtPiece), kPtPiece);
-                    const uint32_t o = tmem + 256 + 128 * s, w = tmem + 128 * s;
-#pragma unroll
-                    for (int k = 0; k < kPtKeys / 16; k++) {
-                        if (f32) umma_bf16_ts(o, w + 64 + 8 * k, vd + (uint64_t)(k * 128), idesc_o, (n > 1) | k ? 1u : 0u);
-                        umma_bf16_ts(o, w + 8 * k, vd + (uint64_t)(k * 128), idesc_o, f32 || (n > 1) | k ? 1u : 0u);
+                            for (int h = 0; h < kHalves; h++)
+                                tma_rows_3d(sq + (s * kHalves + h) * kPtPiece, &qmap, 64 * h, it.head * p.share, it.job.first + it.t0 + s * tile_tokens, &q_full);
                     }
-                    umma_commit(&o_done[s]);
-                    if (!dual || s == 1) umma_commit(&v_empty[slot]);
-                    steps[s]++;
-                    if (n + 2 < n_steps) ok = scores(n + 2);
                 }
-                nk += it.blocks;
+                // a lane per page (box) of a block
+                const int box_rows = p.page < kPtKeys ? p.page : kPtKeys, boxes = kPtKeys / box_rows;
+                const int* table = p.table + (size_t)it.job.seq * p.max_pages;
+                auto entry_of = [&](int b) {
+                    const int key = it.from + b * kPtKeys + lane * box_rows;
+                    return lane < boxes && key < it.job.to ? table[key >> p.log_page] : -2;
+                };
+                int entry = entry_of(0);
+                for (int b = 0; b < it.blocks; b++, nk++) {
+                    const int slot = nk % kDepth, now = entry;
+                    if (b + 1 < it.blocks) entry = entry_of(b + 1);
+                    const bool have = now >= 0 && now < p.n_pages;
+                    if (now != -2 && !have) report(err, 82);
+                    const unsigned who = __ballot_sync(0xFFFFFFFFu, have);
+                    if (nk >= kDepth && !mbar_wait_bounded(&empty[slot], (uint32_t)(nk / kDepth - 1) & 1u, err, 85 + !keys)) { ok = false; break; }
+                    if (lane == 0) {
+                        if (keys) {
+                            unsigned missing = 0;
+                            for (int g = 0; g < 16; g++)
+                                if (!(who >> (g * 8 / box_rows) & 1u)) missing |= 1u << g;
+                            s_missing[nk & 7] = (unsigned short)missing;
+                        }
+                        mbar_expect_tx(&full[slot], (uint32_t)(__popc(who) * box_rows * 128 * kHalves));
+                    }
+                    __syncwarp();
+                    const int row = (it.from + b * kPtKeys + lane * box_rows) & (p.page - 1);
+                    if (have)
+                        for (int h = 0; h < (p.both ? 1 : kHalves); h++)
+                            tma_page(smem_addr(room + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), map, 64 * h, row, it.head, now, smem_addr(&full[slot]));
+                }
             }
-        }
+        } else {
+            // ---------------- MMAs.  (What this thread computes between two products is a chain that nothing covers: addresses and descriptors are ready ahead.)
+            const int s = warp >> 1;
+            if (elect_one()) {
+                constexpr uint32_t kind = std::is_same<K, bf16>::value ? 1u : 0u;
+                constexpr uint32_t fmt = (1u << 4) | (kind << 7) | (kind << 10) | ((uint32_t)(kPtRows >> 4) << 24);
+                constexpr uint32_t idesc_s = fmt | ((uint32_t)(kPtStep >> 3) << 17), idesc_o = fmt | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
+                constexpr uint32_t block = kHalves * kPtPiece >> 4, half_block = kPtStep * 128 >> 4;       // in a descriptor's units
+                const uint32_t o = tmem + 256 + 128 * s, scores_at = tmem + 128 * s;
+                const uint32_t b_s = smem_addr(s_full[s]), b_p = smem_addr(p_full[s]), b_o = smem_addr(o_done[s]), b_kf = smem_addr(k_full), b_ke = smem_addr(k_empty),
+                               b_vf = smem_addr(v_full), b_ve = smem_addr(v_empty);
+                const uint64_t kd0 = swizzled_desc(smem_addr(sk)), vd0 = swizzled_desc_mn(smem_addr(sv), kPtPiece);
+                PtItem it = {};
+                int items = 0;
+                uint32_t ks = 0, kp = 0, vs = 0, vp = 0;        // the next blocks of keys and values: slots and phases
+                uint32_t si = 0, pi = 0;                        // steps so far: scores, sums
+                bool ok = true;
+                for (int u = u0; ok && u < u1; u += it.blocks, items++) {
+                    open(it, u, u != u0);
+                    const bool dual = is_dual(it);
+                    const int steps = dual ? 2 * it.blocks : it.blocks;
+                    const uint64_t qd = swizzled_desc(smem_addr(sq + (dual ? s : 0) * kHalves * kPtPiece));
+                    if (!(ok = mbar_wait_bounded(&q_full, (uint32_t)items & 1u, err, 87))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    // step t reads half `h` of a block; `first` and `last` of this stream's steps on it
+                    auto scores = [&](int t) {
+                        const int h = dual ? t & 1 : s;
+                        const bool first = !dual || !(t & 1), last = !dual || (t & 1);
+                        if (first && !mbar_wait_at(b_kf + 8 * ks, kp, err, 88)) return false;
+                        const uint64_t kd = kd0 + ks * block + h * half_block;
+                        const uint32_t to = scores_at + 64 * (si & 1);
+#pragma unroll
+                        for (int part = 0; part < (f32 ? 2 : 1); part++)
+#pragma unroll
+                            for (int c = 0; c < kHalves; c++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++)
+                                    umma_bf16_ss(to, qd + (uint64_t)((part * kHalves + c) * (kPtPiece >> 4) + 2 * k), kd + (uint64_t)(c * (kPtPiece >> 4) + 2 * k), idesc_s,
+                                                 part | c | k ? 1u : 0u);
+                        umma_commit_at(b_s + 8 * (si & 1));
+                        if (last) {
+                            umma_commit_at(b_ke + 8 * ks);
+                            if (++ks == kDepth) { ks = 0; kp ^= 1; }
+                        }
+                        si++;
+                        if (t == steps - 1) umma_commit(&q_empty);
+                        return true;
+                    };
+                    ok = scores(0) && (steps < 2 || scores(1));
+#pragma unroll 1
+                    for (int t = 0; ok && t < steps; t++) {
+                        const int h = dual ? t & 1 : s;
+                        const bool first = !dual || !(t & 1), last = !dual || (t & 1);
+                        if (first && !(ok = mbar_wait_at(b_vf + 8 * vs, vp, err, 89))) break;
+                        if (!(ok = mbar_wait_at(b_p + 8 * (pi & 1), (pi >> 1) & 1u, err, 90))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t vd = vd0 + vs * block + h * half_block;
+                        const uint32_t w = scores_at + 64 * (pi & 1);
+#pragma unroll
+                        for (int k = 0; k < kPtStep / 16; k++) {
+                            if (f32) umma_bf16_ts(o, w + 32 + 8 * k, vd + (uint64_t)(k * 128), idesc_o, t | k ? 1u : 0u);
+                            umma_bf16_ts(o, w + 8 * k, vd + (uint64_t)(k * 128), idesc_o, f32 || (t | k) ? 1u : 0u);
+                        }
+                        umma_commit_at(b_o + 8 * (pi & 1));
+                        if (last) {
+                            umma_commit_at(b_ve + 8 * vs);
+                            if (++vs == kDepth) { vs = 0; vp ^= 1; }
+                        }
+                        pi++;
+                        if (t + 2 < steps) ok = scores(t + 2);
+                    }
+                }
+            }
         __syncwarp();
         }
     }
