@@ -10,126 +10,123 @@ static int check_groups(const bpdq_paged_kv* kv, const bpdq_paged_groups* g)
     return g && (g->n < 0 || g->n > kv->batch || (g->n && (!g->start || !g->pages))) ? latch(BPDQ_ERR_ARG) : 0;
 }
 
-// Adds up the parts of rows that the kernels ahead have left in scratch memory: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  A warp per row, or four of
-// them where there are few rows.
-template <typename A, int DP, int TEAM>
-__global__ void __launch_bounds__(128) k_paged_join(const PagedArgs p)
+// Adds up the parts of rows that the kernels ahead have left in scratch memory: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  Eight threads walk through the
+// parts of a row; or, where there are few rows, a CTA has one row and eight threads every sixteenth part.
+constexpr int kJoinThreads = 128, kJoinGroups = kJoinThreads / 8;
+
+template <typename A, int DP, bool kFew>
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedArgs p)
 {
-    constexpr int kCols = DP / 32;
-    __shared__ float s_o[4][DP];
-    __shared__ float2 s_ml[4];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = TEAM > 1 ? warp : 0;
-    const long rows = (long)p.n_tokens * p.heads, teams = (long)gridDim.x * (4 / TEAM), team = TEAM > 1 ? (long)blockIdx.x : (long)blockIdx.x * 4 + warp;
+    constexpr int kUnits = DP / 32;
+    __shared__ float s_o[kFew ? kJoinGroups : 1][DP];
+    __shared__ float2 s_ml[kJoinGroups];
+    const int l8 = threadIdx.x & 7, group = threadIdx.x >> 3;
+    const long rows = (long)p.n_tokens * p.heads, stride = kFew ? (long)gridDim.x : (long)gridDim.x * kJoinGroups;
     pdl_wait();
     pdl_launch_dependents();
-    for (long base = team; base < rows; base += 32 * teams) {
-        // the descriptors of the team's next 32 rows at once
-        const long mine = base + lane * teams;
-        int4 d = make_int4(0, 0, 0, 0);
-        if (mine < rows) d = p.own[mine];
-        unsigned todo = __ballot_sync(0xFFFFFFFFu, d.y > 1 || (d.y == 1 && (d.w & kJoinPrefix)));
-        while (todo) {
-            const int src = __ffs(todo) - 1;
-            todo &= todo - 1;
-            const long row = base + src * teams;
-            const int4 own = make_int4(__shfl_sync(0xFFFFFFFFu, d.x, src), __shfl_sync(0xFFFFFFFFu, d.y, src), __shfl_sync(0xFFFFFFFFu, d.z, src), __shfl_sync(0xFFFFFFFFu, d.w, src));
-            int4 pre = make_int4(0, 0, 0, 0);
-            if (own.w & kJoinPrefix) pre = p.prefix[row];
-            // part i of the row: its own positions' first, then the prefix's
-            const int n = own.y + pre.y;
-            auto place = [&](int i, const float*& o, const float2*& ml) {
-                const bool mine = i < own.y;
-                const int4 e = mine ? own : pre;
-                const int k = mine ? i : i - own.y;
-                size_t at;
-                if (e.y == 1) {
-                    at = (size_t)row;
-                    o = mine ? p.own_o : p.prefix_o;
-                    ml = mine ? p.own_ml : p.prefix_ml;
-                } else {
-                    at = (size_t)(2 * (e.x + k) + (k == 0)) * (e.w & kJoinTile ? kTileRows : kSplitRows) + e.z;
-                    o = e.w & kJoinTile ? p.tile_o : p.split_o;
-                    ml = e.w & kJoinTile ? p.tile_ml : p.split_ml;
-                }
-                o += at * DP;
-                ml += at;
-            };
-            float most = -INFINITY, l = 0.0f, acc[kCols];
-#pragma unroll
-            for (int c = 0; c < kCols; c++) acc[c] = 0.0f;
-            // the member's parts: member, member + TEAM, ..; their maxima and sums a lane each, their outputs eight at a time
-            for (int i0 = 0; i0 * TEAM + member < n; i0 += 32) {
-                const int i = (i0 + lane) * TEAM + member;
-                const float* o = p.own_o;
-                const float2* ml = nullptr;
-                float2 v = make_float2(-INFINITY, 0.0f);
-                if (i < n) {
-                    place(i, o, ml);
-                    v = *ml;
-                }
-                const float top = fmaxf(most, warp_max(v.x)), ref = top == -INFINITY ? 0.0f : top, down = ex2(most - ref);
-                const float w = ex2(v.x - ref);
-                l = l * down + warp_sum(w * v.y);
-                most = top;
-#pragma unroll
-                for (int c = 0; c < kCols; c++) acc[c] *= down;
-                const int here = min(32, (n - member + TEAM - 1) / TEAM - i0);
-                for (int k0 = 0; k0 < here; k0 += 8) {
-                    float x[8][kCols];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const float* from = reinterpret_cast<const float*>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)o, k0 + k)) + kCols * lane;
-#pragma unroll
-                        for (int c = 0; c < kCols; c++) x[k][c] = 0.0f;
-                        if (k0 + k < here) {
-                            if constexpr (kCols == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(from);
-                            else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const float wk = __shfl_sync(0xFFFFFFFFu, w, k0 + k);
-#pragma unroll
-                        for (int c = 0; c < kCols; c++) acc[c] = fmaf(wk, x[k][c], acc[c]);
-                    }
-                }
+    long row = kFew ? (long)blockIdx.x : (long)blockIdx.x * kJoinGroups + group;
+    int4 next = row < rows ? p.own[row] : make_int4(0, 0, 0, 0);
+    for (; row < rows; row += stride) {
+        const int4 own = next;
+        if (row + stride < rows) next = p.own[row + stride];
+        if (own.y == 0 || (own.y == 1 && !(own.w & kJoinPrefix))) continue;
+        int4 pre = make_int4(0, 0, 0, 0);
+        if (own.w & kJoinPrefix) pre = p.prefix[row];
+        // part i of the row: its own positions' first, then the prefix's
+        const int n = own.y + pre.y;
+        auto place = [&](int i, const float*& o, const float2*& ml) {
+            const bool mine = i < own.y;
+            const int4 e = mine ? own : pre;
+            const int k = mine ? i : i - own.y;
+            size_t at = (size_t)row;
+            if (e.y == 1) {
+                o = mine ? p.own_o : p.prefix_o;
+                ml = mine ? p.own_ml : p.prefix_ml;
+            } else {
+                at = (size_t)(2 * (e.x + k) + (k == 0)) * (e.w & kJoinTile ? kTileRows : kSplitRows) + e.z;
+                o = e.w & kJoinTile ? p.tile_o : p.split_o;
+                ml = e.w & kJoinTile ? p.tile_ml : p.split_ml;
             }
-            if (TEAM > 1) {
-                __syncthreads();                    // (what the row before was read from)
-                if (lane == 0) s_ml[warp] = make_float2(most, l);
+            o += at * DP + 4 * l8;
+            ml += at;
+        };
+        float top = -INFINITY, l = 0.0f;
+        float4 acc[kUnits];
 #pragma unroll
-                for (int c = 0; c < kCols; c++) s_o[warp][kCols * lane + c] = acc[c];
-                __syncthreads();
-                if (warp > 0) continue;
-                float top = -INFINITY;
-                for (int i = 0; i < TEAM; i++) top = fmaxf(top, s_ml[i].x);
-                const float ref = top == -INFINITY ? 0.0f : top;
-                l = 0.0f;
+        for (int c = 0; c < kUnits; c++) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // two parts at a time
+        constexpr int step = kFew ? kJoinGroups : 1;
+#pragma unroll 1
+        for (int i = kFew ? group : 0; i < n; i += 2 * step) {
+            const float* o[2];
+            const float2* ml[2];
+            float2 v[2];
+            float4 x[2][kUnits];
+            const bool two = i + step < n;
+            place(i, o[0], ml[0]);
+            place(two ? i + step : i, o[1], ml[1]);
 #pragma unroll
-                for (int c = 0; c < kCols; c++) acc[c] = 0.0f;
-                for (int i = 0; i < TEAM; i++) {
-                    const float w = ex2(s_ml[i].x - ref);
-                    l = fmaf(w, s_ml[i].y, l);
+            for (int k = 0; k < 2; k++) {
+                v[k] = *ml[k];
 #pragma unroll
-                    for (int c = 0; c < kCols; c++) acc[c] = fmaf(w, s_o[i][kCols * lane + c], acc[c]);
-                }
+                for (int c = 0; c < kUnits; c++) x[k][c] = *reinterpret_cast<const float4*>(o[k] + 32 * c);
             }
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            A* out = static_cast<A*>(p.o) + (size_t)(row / p.heads) * p.ld_o + (int)(row % p.heads) * p.dim;
+            if (!two) v[1] = make_float2(-INFINITY, 0.0f);
+            const float now = fmaxf(top, fmaxf(v[0].x, v[1].x)), zero = now == -INFINITY ? 0.0f : now;
+            const float down = ex2(top - zero), w0 = ex2(v[0].x - zero), w1 = ex2(v[1].x - zero);
+            l = fmaf(w1, v[1].y, fmaf(w0, v[0].y, l * down));
+            top = now;
 #pragma unroll
-            for (int c = 0; c < kCols; c++)
-                if (kCols * lane + c < p.dim) out[kCols * lane + c] = ActOf<A>::put(acc[c] * inv);
+            for (int c = 0; c < kUnits; c++) {
+                acc[c].x = fmaf(w1, x[1][c].x, fmaf(w0, x[0][c].x, acc[c].x * down));
+                acc[c].y = fmaf(w1, x[1][c].y, fmaf(w0, x[0][c].y, acc[c].y * down));
+                acc[c].z = fmaf(w1, x[1][c].z, fmaf(w0, x[0][c].z, acc[c].z * down));
+                acc[c].w = fmaf(w1, x[1][c].w, fmaf(w0, x[0][c].w, acc[c].w * down));
+            }
         }
+        A* out = static_cast<A*>(p.o) + (size_t)(row / p.heads) * p.ld_o + (int)(row % p.heads) * p.dim;
+        if (kFew) {
+            __syncthreads();                    // (what the row before was read from)
+            if (l8 == 0) s_ml[group] = make_float2(top, l);
+#pragma unroll
+            for (int c = 0; c < kUnits; c++) *reinterpret_cast<float4*>(&s_o[kFew ? group : 0][32 * c + 4 * l8]) = acc[c];
+            __syncthreads();
+            const int d = threadIdx.x;
+            if (d < p.dim) {
+                const int used = n < kJoinGroups ? n : kJoinGroups;
+                float most = -INFINITY, sum = 0.0f, o = 0.0f;
+                for (int i = 0; i < used; i++) most = fmaxf(most, s_ml[i].x);
+                const float zero = most == -INFINITY ? 0.0f : most;
+                for (int i = 0; i < used; i++) {
+                    const float w = ex2(s_ml[i].x - zero);
+                    sum = fmaf(w, s_ml[i].y, sum);
+                    o = fmaf(w, s_o[kFew ? i : 0][d], o);
+                }
+                out[d] = ActOf<A>::put(sum > 0.0f ? o / sum : 0.0f);
+            }
+            continue;
+        }
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int c = 0; c < kUnits; c++)
+            if (32 * c + 4 * l8 < p.dim) {
+                A* at = out + 32 * c + 4 * l8;
+                at[0] = ActOf<A>::put(acc[c].x * inv);
+                at[1] = ActOf<A>::put(acc[c].y * inv);
+                at[2] = ActOf<A>::put(acc[c].z * inv);
+                at[3] = ActOf<A>::put(acc[c].w * inv);
+            }
     }
 }
 
 template <typename A, int DP>
 static int launch_join(const PagedArgs& p, cudaStream_t s)
 {
-    const long rows = (long)p.n_tokens * p.heads, room = 8L * sm_count();
-    if (rows <= room) return launch_ordered(k_paged_join<A, DP, 4>, dim3((unsigned)rows), 128, 0, s, p);
-    const long ctas = (rows + 3) / 4;
-    return launch_ordered(k_paged_join<A, DP, 1>, dim3((unsigned)(ctas < room ? ctas : room)), 128, 0, s, p);
+    const long rows = (long)p.n_tokens * p.heads;
+    // a CTA per row: few rows have many parts, and so may rows with a prefix
+    if (rows <= (p.groups ? 16L : 4L) * sm_count()) return launch_ordered(k_paged_join<A, DP, true>, dim3((unsigned)rows), kJoinThreads, 0, s, p);
+    const long ctas = (rows + kJoinGroups - 1) / kJoinGroups, room = 12L * sm_count();
+    return launch_ordered(k_paged_join<A, DP, false>, dim3((unsigned)(ctas < room ? ctas : room)), kJoinThreads, 0, s, p);
 }
 
 // Scratch of a call, carved out of `base` (null: sizes alone); returns its bytes.
@@ -188,8 +185,11 @@ struct Kernels {
 };
 static Kernels kernels(const PagedArgs& p)
 {
+    // k_paged_split's products of 8 rows or of 16: of 16 where sequences bring between 8 and 16 on average (a few tokens each), which the larger tiles would
+    // be mostly empty with.
+    const long average = p.seq_start ? ((long)p.n_tokens * p.share + p.batch - 1) / p.batch : p.share;
     Kernels k;
-    k.split_rows = p.share > kSplitRows ? 0 : (p.share <= 8 && !p.seq_start ? 8 : kSplitRows);
+    k.split_rows = p.share > kSplitRows ? 0 : (p.share > 8 || (average > 8 && average <= kSplitRows) ? kSplitRows : 8);
     k.tile = p.seq_start || p.groups || !k.split_rows;
     return k;
 }

@@ -383,75 +383,79 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     if (p.mark && warp == kPsWarps - 1) mark_tokens(p, lane, 32, err);
     __syncthreads();
 
-    // ---- items that several warps have parts of, each row by a warp.  Part e is the first (e even) or last part of warp e / 2.
-    constexpr int kCols = DP / 32;
-    const PsPart* part = &parts[(lane & 15) >> 1][lane & 1];
-    const unsigned exist = __ballot_sync(0xFFFFFFFFu, lane < 2 * kPsWarps && part->valid);
-    const int begins = part->begin, before = exist & ((1u << lane) - 1) ? 31 - __clz(exist & ((1u << lane) - 1)) : lane;
+    // ---- items that several warps have parts of, eight threads per row.  Part e is the first (e even) or last part of warp e / 2.
+    const PsPart* of_lane = &parts[(lane & 15) >> 1][lane & 1];
+    const unsigned exist = __ballot_sync(0xFFFFFFFFu, lane < 2 * kPsWarps && of_lane->valid);
+    const int begins = of_lane->begin, before = exist & ((1u << lane) - 1) ? 31 - __clz(exist & ((1u << lane) - 1)) : lane;
     const int begins_before = __shfl_sync(0xFFFFFFFFu, begins, before);
     unsigned heads = __ballot_sync(0xFFFFFFFFu, (exist >> lane & 1u) && (before == lane || begins_before != begins));        // the items' first parts
-    for (int turn = 0; heads;) {
+    const int l8 = tid & 7;
+    int turn = tid >> 3;                // the rows, item by item, that are still to be passed over
+#pragma unroll 1
+    while (heads) {
         const int e = __ffs(heads) - 1;
         heads &= heads - 1;
-        const unsigned members = exist & ~((1u << e) - 1) & (heads ? (1u << (__ffs(heads) - 1)) - 1 : ~0u);
         const PsPart item = parts[e >> 1][e & 1];
+        if (turn >= item.rows) { turn -= item.rows; continue; }
+        const unsigned members = exist & ~((1u << e) - 1) & (heads ? (1u << (__ffs(heads) - 1)) - 1 : ~0u);
         const bool starts = item.begin >= u0, all = starts && item.end <= u1;
-        for (int r = 0; r < item.rows; r++) {
-            if (turn++ % kPsWarps != warp) continue;
-            // a lane per part: its maximum and sum
-            const int w = (lane & 15) >> 1;
-            float2 v = make_float2(-INFINITY, 0.0f);
-            if (members >> lane & 1u)
-                v = lane & 1 ? reinterpret_cast<const float2*>(reinterpret_cast<const float*>(ring_ptr + w * kPsRing) + kSplitRows * DP)[r]
-                             : p.head_ml[(size_t)(cta * kPsWarps + w) * kSplitRows + r];
-            const float top = warp_max(v.x), weight = ex2(v.x - (top == -INFINITY ? 0.0f : top)), l = warp_sum(weight * v.y);
-            float acc[kCols];
+        const int r = turn;
+        turn += kPsThreads / 8 - item.rows;         // (an item has fewer rows than there are groups of threads)
+        float top = -INFINITY, l = 0.0f;
+        float4 acc[kHalves * 2];
 #pragma unroll
-            for (int c = 0; c < kCols; c++) acc[c] = 0.0f;
-            unsigned rest = members;
+        for (int c = 0; c < kHalves * 2; c++) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // two parts at a time
 #pragma unroll 1
-            while (rest) {
-                // two parts at a time
-                float x[2][kCols], wi[2];
+        for (unsigned rest = members; rest;) {
+            float2 v[2];
+            float4 x[2][kHalves * 2];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int i = rest ? __ffs(rest) - 1 : 0;
-                    wi[k] = __shfl_sync(0xFFFFFFFFu, weight, i);
+            for (int k = 0; k < 2; k++) {
+                const int i = rest ? __ffs(rest) - 1 : e;
+                const size_t at = (size_t)(cta * kPsWarps + (i >> 1)) * kSplitRows;
+                const float* ring_part = reinterpret_cast<const float*>(ring_ptr + (i >> 1) * kPsRing);
+                const float* from = (i & 1 ? ring_part : p.head_o + at * DP) + r * DP + 4 * l8;
+                v[k] = i & 1 ? reinterpret_cast<const float2*>(ring_part + kSplitRows * DP)[r] : p.head_ml[at + r];
 #pragma unroll
-                    for (int c = 0; c < kCols; c++) x[k][c] = 0.0f;
-                    if (rest) {
-                        const float* from = (i & 1 ? reinterpret_cast<const float*>(ring_ptr + (i >> 1) * kPsRing) : p.head_o + (size_t)(cta * kPsWarps + (i >> 1)) * kSplitRows * DP) +
-                                            r * DP + kCols * lane;
-                        if constexpr (kCols == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(from);
-                        else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
-                    }
-                    rest &= rest - 1;
+                for (int c = 0; c < kHalves * 2; c++) x[k][c] = *reinterpret_cast<const float4*>(from + 32 * c);
+                if (!rest) v[k] = make_float2(-INFINITY, 0.0f);
+                rest &= rest - 1;
+            }
+            const float now = fmaxf(top, fmaxf(v[0].x, v[1].x)), zero = now == -INFINITY ? 0.0f : now;
+            const float down = ex2(top - zero), w0 = ex2(v[0].x - zero), w1 = ex2(v[1].x - zero);
+            l = fmaf(w1, v[1].y, fmaf(w0, v[0].y, l * down));
+            top = now;
+#pragma unroll
+            for (int c = 0; c < kHalves * 2; c++) {
+                acc[c].x = fmaf(w1, x[1][c].x, fmaf(w0, x[0][c].x, acc[c].x * down));
+                acc[c].y = fmaf(w1, x[1][c].y, fmaf(w0, x[0][c].y, acc[c].y * down));
+                acc[c].z = fmaf(w1, x[1][c].z, fmaf(w0, x[0][c].z, acc[c].z * down));
+                acc[c].w = fmaf(w1, x[1][c].w, fmaf(w0, x[0][c].w, acc[c].w * down));
+            }
+        }
+        const int t = r / p.share, tok = item.first + t, h = item.head * p.share + r - t * p.share;
+        const size_t row = (size_t)tok * p.heads + h;
+        if (all && !item.joined) {
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            A* out_row = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim + 4 * l8;
+#pragma unroll
+            for (int c = 0; c < kHalves * 2; c++)
+                if (32 * c + 4 * l8 < p.dim) {
+                    store_two<A>(out_row + 32 * c, acc[c].x * inv, acc[c].y * inv);
+                    store_two<A>(out_row + 32 * c + 2, acc[c].z * inv, acc[c].w * inv);
                 }
+        } else {
+            const size_t at = all ? row : (size_t)(2 * cta + starts) * kSplitRows + r;
+            float* dst = (!all ? p.split_o : (item.prefix ? p.prefix_o : p.own_o)) + at * DP + 4 * l8;
 #pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int c = 0; c < kCols; c++) acc[c] = fmaf(wi[k], x[k][c], acc[c]);
-            }
-            const int t = r / p.share, tok = item.first + t, h = item.head * p.share + r - t * p.share;
-            const size_t row = (size_t)tok * p.heads + h;
-            if (all && !item.joined) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                A* out_row = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim;
-#pragma unroll
-                for (int c = 0; c < kCols; c += 2)
-                    if (kCols * lane + c < p.dim) store_two<A>(out_row + kCols * lane + c, acc[c] * inv, acc[c + 1] * inv);
-            } else {
-                const size_t at = all ? row : (size_t)(2 * cta + starts) * kSplitRows + r;
-                float* dst = (!all ? p.split_o : (item.prefix ? p.prefix_o : p.own_o)) + at * DP + kCols * lane;
-#pragma unroll
-                for (int c = 0; c < kCols; c += 2) store_two<float>(dst + c, acc[c], acc[c + 1]);
-                if (lane == 0) (!all ? p.split_ml : (item.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top, l);
-            }
-            if (lane == 0 && starts) {
-                // the CTA with the item's last unit
-                const int end = all ? cta : deal.cta_of(item.end - 1);
-                (item.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, r, item.joined && !item.prefix ? kJoinPrefix : 0);
-            }
+            for (int c = 0; c < kHalves * 2; c++) *reinterpret_cast<float4*>(dst + 32 * c) = acc[c];
+            if (l8 == 0) (!all ? p.split_ml : (item.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top, l);
+        }
+        if (l8 == 0 && starts) {
+            // the CTA with the item's last unit
+            const int end = all ? cta : deal.cta_of(item.end - 1);
+            (item.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, r, item.joined && !item.prefix ? kJoinPrefix : 0);
         }
     }
 }

@@ -92,8 +92,11 @@ struct PtItem {
     PagedJob job;
     int j, head, begin, end;            // units: its blocks of keys
     int t0, tokens;                     // the first token, within the job, and how many
-    int from, blocks;                   // position of the first key
+    int from, blocks, units;            // this CTA's part of it: position of the first key, blocks, units
+    bool starts;                        // it has the item's first block
 };
+// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as a block: it counts a unit more than it has blocks, its first.
+constexpr int kPtExtra = 1;
 
 template <typename A, typename K, int DP>
 __global__ void __launch_bounds__(kPtThreads, 1)
@@ -118,7 +121,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     }
     if (tid == 0) {
         mbar_init(&q_full, f32 ? kPtWarps : 1);
-        mbar_init(&q_empty, 2);
+        mbar_init(&q_empty, kPtWarps);
         for (int i = 0; i < kDepth; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 2); }
         for (int i = 0; i < 2; i++) { mbar_init(&s_full[0][i], 1); mbar_init(&s_full[1][i], 1); mbar_init(&p_full[0][i], 4); mbar_init(&p_full[1][i], 4); mbar_init(&o_done[0][i], 1); mbar_init(&o_done[1][i], 1); }
         mbar_init(&ml_ready, 4);
@@ -148,7 +151,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     const int total = plan.build<kPtThreads>(p, reinterpret_cast<int*>(base + Shape::end), err, [&](const PagedJob& r) {
         if (r.rows <= p.split_rows) return 0;
         int n = 0;
-        for (int t = 0; t < r.count; t += item_tokens) n += blocks_of(r, t);
+        for (int t = 0; t < r.count; t += item_tokens) n += blocks_of(r, t) + kPtExtra;
         return n;
     });
     const int ctas = max(1, min((int)gridDim.x, total)), cta = blockIdx.x;
@@ -164,17 +167,20 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         it.head = at / per;
         at -= it.head * per;
         it.t0 = 0;
-        int n = blocks_of(it.job, 0);
+        int n = blocks_of(it.job, 0) + kPtExtra;
         while (at >= n) {
             at -= n;
             it.t0 += item_tokens;
-            n = blocks_of(it.job, it.t0);
+            n = blocks_of(it.job, it.t0) + kPtExtra;
         }
         it.begin = u - at;
         it.end = it.begin + n;
+        it.units = min(it.end, u1) - u;
         it.tokens = min(item_tokens, it.job.count - it.t0);
-        it.from = it.job.from + at * kPtKeys;
-        it.blocks = min(it.end, u1) - u;
+        const int block = max(at - kPtExtra, 0);
+        it.from = it.job.from + block * kPtKeys;
+        it.blocks = at + it.units - kPtExtra - block;           // (none: the next CTA has the first one)
+        it.starts = block == 0;
     };
     // Two tiles, each against every block, step t against half t % 2 of block t / 2; or one, stream s against half s of block t.
     auto is_dual = [&](const PtItem& it) { return !f32 && it.tokens > tile_tokens; };
@@ -188,8 +194,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         PtItem it = {};
         int nk = 0, steps = 0, items = 0, meets = 0;
         bool ok = true;
-        for (int u = u0; ok && u < u1; u += it.blocks, items++) {
+        for (int u = u0; ok && u < u1; u += it.units) {
             open(it, u, u != u0);
+            if (it.blocks <= 0) continue;
             const bool dual = is_dual(it);
             const int n_steps = dual ? 2 * it.blocks : it.blocks;
             const int mine = (dual ? s * tile_tokens : 0) + r / p.share;            // the row's token, within the item
@@ -347,6 +354,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     // its sums are read by the other stream's threads
                     if (!mbar_wait_bounded(&o1_free, (uint32_t)meets & 1u, err, 96)) { ok = false; break; }
                     meets++;
+                    items++;
+                    if (lane == 0) mbar_arrive(&q_empty);
                     continue;
                 }
                 if (!mbar_wait_bounded(&ml_ready, (uint32_t)meets & 1u, err, 97)) { ok = false; break; }
@@ -361,47 +370,61 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     top = most;
                 }
             }
-            const bool starts = it.begin >= u0, all = starts && it.end <= u1;
+            const bool starts = it.starts, all = starts && it.end <= u1;
             const size_t row = (size_t)tok * p.heads + h;
             const int in_part = (dual ? s * kPtRows : 0) + r;
             const size_t at = all ? row : (size_t)(2 * cta + starts) * kTileRows + in_part;
             const bool direct = all && !it.job.joined;
-            float* dst = (!all ? p.tile_o : (it.job.prefix ? p.prefix_o : p.own_o)) + at * DP;
-            A* o = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim;
             if (direct) {
                 const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
                 w0 *= inv;
                 w1 *= inv;
             }
+            // Rows pass through the room of the item's queries, of which a warp has an eighth, so that whole lines of them are stored: DP * 2 bytes of a row at a time, 16-byte
+            // units turned by the row.
+            constexpr int kUnits = DP / 8;
+            uint8_t *room = sq + (s * 4 + quarter) * (32 * DP * 2), *mine_room = room + lane * DP * 2;
+            uint8_t* dst = direct ? reinterpret_cast<uint8_t*>(static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim)
+                                  : reinterpret_cast<uint8_t*>((!all ? p.tile_o : (it.job.prefix ? p.prefix_o : p.own_o)) + at * DP);
+            const bool narrow = direct && !f32;             // 16-bit results
+            const int row_bytes = direct ? p.dim * (int)sizeof(A) : DP * 4, pass = narrow ? DP : DP / 2;
+            const unsigned alive = __ballot_sync(0xFFFFFFFFu, live);
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
-                float x[32];
-                tmem_ld_32(to_ + 128 * s + c, x);
-                if (!dual) {
-                    float y[32];
-                    tmem_ld_32(to_ + 128 + c, y);
-                    tmem_loaded();
+            for (int c0 = 0; c0 < DP; c0 += pass) {
+#pragma unroll 1
+                for (int c = c0; c < c0 + pass; c += 32) {
+                    float x[32];
+                    tmem_ld_32(to_ + 128 * s + c, x);
+                    if (!dual) {
+                        float y[32];
+                        tmem_ld_32(to_ + 128 + c, y);
+                        tmem_loaded();
 #pragma unroll
-                    for (int j = 0; j < 32; j++) x[j] = fmaf(y[j], w1, x[j] * w0);
-                } else {
-                    tmem_loaded();
+                        for (int j = 0; j < 32; j++) x[j] = fmaf(y[j], w1, x[j] * w0);
+                    } else {
+                        tmem_loaded();
 #pragma unroll
-                    for (int j = 0; j < 32; j++) x[j] *= w0;
+                        for (int j = 0; j < 32; j++) x[j] *= w0;
+                    }
+                    if (narrow) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            *reinterpret_cast<uint4*>(mine_room + (((((c - c0) >> 3) + j) ^ (lane & (kUnits - 1))) << 4)) =
+                                make_uint4(pack_16<K>(x[8 * j], x[8 * j + 1]), pack_16<K>(x[8 * j + 2], x[8 * j + 3]), pack_16<K>(x[8 * j + 4], x[8 * j + 5]), pack_16<K>(x[8 * j + 6], x[8 * j + 7]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            *reinterpret_cast<float4*>(mine_room + (((((c - c0) >> 2) + j) ^ (lane & (kUnits - 1))) << 4)) = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+                    }
                 }
-                if (!live) {
-                } else if (!direct) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(dst + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-                } else if constexpr (f32) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        if (c + j < p.dim) *reinterpret_cast<float4*>(o + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        if (c + j < p.dim)
-                            *reinterpret_cast<uint4*>(o + c + j) = make_uint4(pack_16<K>(x[j], x[j + 1]), pack_16<K>(x[j + 2], x[j + 3]), pack_16<K>(x[j + 4], x[j + 5]),
-                                                                              pack_16<K>(x[j + 6], x[j + 7]));
+                __syncwarp();
+                const int unit = lane & (kUnits - 1), byte = c0 * (narrow ? 2 : 4) + 16 * unit;
+#pragma unroll 4
+                for (int i = 0; i < kUnits; i++) {
+                    const int from = i * (32 / kUnits) + lane / kUnits;
+                    uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)dst, from));
+                    const uint4 x = *reinterpret_cast<const uint4*>(room + from * DP * 2 + ((unit ^ (from & (kUnits - 1))) << 4));
+                    if ((alive >> from & 1u) && byte < row_bytes) *reinterpret_cast<uint4*>(to + byte) = x;
                 }
                 __syncwarp();
             }
@@ -413,8 +436,13 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // (the next queries are copied there)
             __syncwarp();
+            if (lane == 0) mbar_arrive(&q_empty);
             if (!dual && lane == 0) mbar_arrive(&o1_free);
+            // the stream's other warps may still read where this one will put queries
+            if (f32 && !mbar_wait_bounded(&o1_free, (uint32_t)(meets - 1) & 1u, err, 99)) { ok = false; break; }
+            items++;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -427,8 +455,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             PtItem it = {};
             int nk = 0, items = 0;
             bool ok = true;
-            for (int u = u0; ok && u < u1; u += it.blocks, items++) {
+            for (int u = u0; ok && u < u1; u += it.units) {
                 open(it, u, u != u0);
+                if (it.blocks <= 0) continue;
                 if (!f32 && keys) {
                     const int tiles = is_dual(it) ? 2 : 1;
                     if (items && !mbar_wait_bounded(&q_empty, (uint32_t)(items - 1) & 1u, err, 84)) break;
@@ -470,6 +499,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         for (int h = 0; h < (p.both ? 1 : kHalves); h++)
                             tma_page(smem_addr(room + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), map, 64 * h, row, it.head, now, smem_addr(&full[slot]));
                 }
+                items++;
             }
         } else {
             // ---------------- MMAs.  (What this thread computes between two products is a chain that nothing covers: addresses and descriptors are ready ahead.)
@@ -488,8 +518,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 uint32_t ks = 0, kp = 0, vs = 0, vp = 0;        // the next blocks of keys and values: slots and phases
                 uint32_t si = 0, pi = 0;                        // steps so far: scores, sums
                 bool ok = true;
-                for (int u = u0; ok && u < u1; u += it.blocks, items++) {
+                for (int u = u0; ok && u < u1; u += it.units) {
                     open(it, u, u != u0);
+                    if (it.blocks <= 0) continue;
                     const bool dual = is_dual(it);
                     const int steps = dual ? 2 * it.blocks : it.blocks;
                     const uint64_t qd = swizzled_desc(smem_addr(sq + (dual ? s : 0) * kHalves * kPtPiece));
@@ -516,7 +547,6 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                             if (++ks == kDepth) { ks = 0; kp ^= 1; }
                         }
                         si++;
-                        if (t == steps - 1) umma_commit(&q_empty);
                         return true;
                     };
                     ok = scores(0) && (steps < 2 || scores(1));
@@ -542,6 +572,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         pi++;
                         if (t + 2 < steps) ok = scores(t + 2);
                     }
+                    items++;
                 }
             }
         __syncwarp();
