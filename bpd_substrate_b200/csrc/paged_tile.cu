@@ -90,13 +90,15 @@ __device__ __forceinline__ float2 ex2_two(float2 x)
 // An item: a key head's rows of some tokens of a job.
 struct PtItem {
     PagedJob job;
-    int j, head, begin, end;            // units: its blocks of keys
+    int head, begin, end;               // units: its blocks of keys
     int t0, tokens;                     // the first token, within the job, and how many
-    int from, blocks, units;            // this CTA's part of it: position of the first key, blocks, units
+    int from, blocks;                   // this CTA's part of it: position of the first key, blocks (0: there are no more items)
     bool starts;                        // it has the item's first block
 };
-// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as a block: it counts a unit more than it has blocks, its first.
-constexpr int kPtExtra = 1;
+constexpr int kPtItems = 4;             // a warp finds the items and puts them here; the others take them
+constexpr int kPtTakers = 1 + 2 + 8;
+// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as two blocks: it counts two units more than it has blocks, its first ones.  (Eight prompts' worth of 8000 tokens: none 692 us, one 595, two 555, three 555, eight 592.)
+constexpr int kPtExtra = 2;
 
 template <typename A, typename K, int DP>
 __global__ void __launch_bounds__(kPtThreads, 1)
@@ -107,9 +109,12 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     constexpr int kHalves = Shape::halves, kDepth = Shape::depth;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t q_full, q_empty, k_full[kDepth], k_empty[kDepth], v_full[kDepth], v_empty[kDepth], s_full[2][2], p_full[2][2], o_done[2][2], ml_ready, o1_free, turn[2];
+    __shared__ uint64_t item_full[kPtItems], item_empty[kPtItems];
+    __shared__ PtItem items[kPtItems];
     __shared__ uint32_t tmem_slot;
     __shared__ unsigned short s_missing[8];             // of a block: groups of eight keys without a page; softmax is two blocks behind the copies' kDepth at most
     __shared__ float2 s_ml[kPtRows];
+    __shared__ uint8_t* s_row[2][kPtRows];              // where rows go; null: nowhere
     __shared__ float s_factor[kPtRows];
     uint8_t* base = raw + (((smem_addr(raw) + 1023) & ~1023u) - smem_addr(raw));
     uint8_t *sq = base + Shape::q, *sk = base + Shape::k, *sv = base + Shape::v;
@@ -124,6 +129,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         mbar_init(&q_empty, kPtWarps);
         for (int i = 0; i < kDepth; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 2); }
         for (int i = 0; i < 2; i++) { mbar_init(&s_full[0][i], 1); mbar_init(&s_full[1][i], 1); mbar_init(&p_full[0][i], 4); mbar_init(&p_full[1][i], 4); mbar_init(&o_done[0][i], 1); mbar_init(&o_done[1][i], 1); }
+        for (int i = 0; i < kPtItems; i++) { mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], kPtTakers); }
         mbar_init(&ml_ready, 4);
         mbar_init(&o1_free, 4);
         mbar_init(&turn[0], 4); mbar_init(&turn[1], 4);
@@ -157,30 +163,14 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     const int ctas = max(1, min((int)gridDim.x, total)), cta = blockIdx.x;
     const PagedDeal deal(total, ctas);
     const int u0 = cta < ctas ? deal.first(cta) : total, u1 = cta < ctas ? deal.first(cta + 1) : total;
-    auto open = [&](PtItem& it, int u, bool again) {
-        if (!again || u >= plan.cum[it.j + 1]) {
-            it.j = plan.find(u);
-            it.job = plan.known(p, it.j);
-        }
-        const int per = (plan.cum[it.j + 1] - plan.cum[it.j]) / p.kv_heads;
-        int at = u - plan.cum[it.j];
-        it.head = at / per;
-        at -= it.head * per;
-        it.t0 = 0;
-        int n = blocks_of(it.job, 0) + kPtExtra;
-        while (at >= n) {
-            at -= n;
-            it.t0 += item_tokens;
-            n = blocks_of(it.job, it.t0) + kPtExtra;
-        }
-        it.begin = u - at;
-        it.end = it.begin + n;
-        it.units = min(it.end, u1) - u;
-        it.tokens = min(item_tokens, it.job.count - it.t0);
-        const int block = max(at - kPtExtra, 0);
-        it.from = it.job.from + block * kPtKeys;
-        it.blocks = at + it.units - kPtExtra - block;           // (none: the next CTA has the first one)
-        it.starts = block == 0;
+    // Item n of this CTA, by a warp (or the thread that issues products).
+    auto take = [&](PtItem& it, int n, bool one) {
+        const int slot = n % kPtItems;
+        if (!mbar_wait_bounded(&item_full[slot], (uint32_t)(n / kPtItems) & 1u, err, 100)) return false;
+        it = items[slot];
+        if (!one) __syncwarp();
+        if (one || lane == 0) mbar_arrive(&item_empty[slot]);
+        return it.blocks > 0;
     };
     // Two tiles, each against every block, step t against half t % 2 of block t / 2; or one, stream s against half s of block t.
     auto is_dual = [&](const PtItem& it) { return !f32 && it.tokens > tile_tokens; };
@@ -192,11 +182,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         const int s = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16, to_ = tmem + lanes + 256;
         PtItem it = {};
-        int nk = 0, steps = 0, items = 0, meets = 0;
+        int nk = 0, steps = 0, taken = 0, meets = 0;
         bool ok = true;
-        for (int u = u0; ok && u < u1; u += it.units) {
-            open(it, u, u != u0);
-            if (it.blocks <= 0) continue;
+        while (ok && take(it, taken, false)) {
             const bool dual = is_dual(it);
             const int n_steps = dual ? 2 * it.blocks : it.blocks;
             const int mine = (dual ? s * tile_tokens : 0) + r / p.share;            // the row's token, within the item
@@ -235,11 +223,13 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
                 // all factors are written
-                if (!mbar_wait_bounded(&q_full, (uint32_t)items & 1u, err, 91)) { ok = false; break; }
+                if (!mbar_wait_bounded(&q_full, (uint32_t)taken & 1u, err, 91)) { ok = false; break; }
                 f *= s_factor[r];
             }
             const float sign = f < 0.0f ? -1.0f : 1.0f;
             f = fabsf(f);
+            const bool plain = p.cap <= 0.0f && __all_sync(0xFFFFFFFFu, sign > 0.0f);
+            const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             float top = -INFINITY, sum = 0.0f;          // in units of log2
             for (int t = 0; t < n_steps; t++, steps++) {
                 const int b = dual ? t >> 1 : t, half = dual ? t & 1 : s, key = it.from + b * kPtKeys + half * kPtStep;
@@ -251,16 +241,17 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 tmem_ld_32(ts + 32, v + 32);
                 tmem_loaded();
                 const unsigned missing = s_missing[(nk + b) & 7] >> (8 * half) & 0xFFu;
-                const bool edge = __any_sync(0xFFFFFFFFu, key + kPtStep > limit || missing);
+                const bool edge = key + kPtStep > least || missing;
                 float ff = f;
-                if (p.cap > 0.0f) {
+                if (plain) {
+                } else if (p.cap > 0.0f) {
                     const float in = sign * f * 0.69314718055994531f;
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[j] = capped<f32>(v[j] * in, p.cap) * 1.44269504088896341f;
                     ff = 1.0f;
-                } else if (sign < 0.0f) {
+                } else {
 #pragma unroll
-                    for (int j = 0; j < 64; j++) v[j] = -v[j];
+                    for (int j = 0; j < 64; j++) v[j] *= sign;
                 }
                 if (edge) {
 #pragma unroll
@@ -354,7 +345,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     // its sums are read by the other stream's threads
                     if (!mbar_wait_bounded(&o1_free, (uint32_t)meets & 1u, err, 96)) { ok = false; break; }
                     meets++;
-                    items++;
+                    taken++;
                     if (lane == 0) mbar_arrive(&q_empty);
                     continue;
                 }
@@ -388,33 +379,30 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                   : reinterpret_cast<uint8_t*>((!all ? p.tile_o : (it.job.prefix ? p.prefix_o : p.own_o)) + at * DP);
             const bool narrow = direct && !f32;             // 16-bit results
             const int row_bytes = direct ? p.dim * (int)sizeof(A) : DP * 4, pass = narrow ? DP : DP / 2;
-            const unsigned alive = __ballot_sync(0xFFFFFFFFu, live);
+            s_row[s][r] = live ? dst : nullptr;
 #pragma unroll 1
             for (int c0 = 0; c0 < DP; c0 += pass) {
 #pragma unroll 1
-                for (int c = c0; c < c0 + pass; c += 32) {
-                    float x[32];
-                    tmem_ld_32(to_ + 128 * s + c, x);
-                    if (!dual) {
-                        float y[32];
-                        tmem_ld_32(to_ + 128 + c, y);
-                        tmem_loaded();
+                for (int c = c0; c < c0 + pass; c += 16) {
+                    int x[16], y[16];
+                    tmem_ld(to_ + 128 * s + c, x);
+                    if (!dual) tmem_ld(to_ + 128 + c, y);
+                    tmem_loaded();
+                    float o[16];
 #pragma unroll
-                        for (int j = 0; j < 32; j++) x[j] = fmaf(y[j], w1, x[j] * w0);
-                    } else {
-                        tmem_loaded();
-#pragma unroll
-                        for (int j = 0; j < 32; j++) x[j] *= w0;
+                    for (int j = 0; j < 16; j++) {
+                        o[j] = __int_as_float(x[j]) * w0;
+                        if (!dual) o[j] = fmaf(__int_as_float(y[j]), w1, o[j]);
                     }
                     if (narrow) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
+                        for (int j = 0; j < 2; j++)
                             *reinterpret_cast<uint4*>(mine_room + (((((c - c0) >> 3) + j) ^ (lane & (kUnits - 1))) << 4)) =
-                                make_uint4(pack_16<K>(x[8 * j], x[8 * j + 1]), pack_16<K>(x[8 * j + 2], x[8 * j + 3]), pack_16<K>(x[8 * j + 4], x[8 * j + 5]), pack_16<K>(x[8 * j + 6], x[8 * j + 7]));
+                                make_uint4(pack_16<K>(o[8 * j], o[8 * j + 1]), pack_16<K>(o[8 * j + 2], o[8 * j + 3]), pack_16<K>(o[8 * j + 4], o[8 * j + 5]), pack_16<K>(o[8 * j + 6], o[8 * j + 7]));
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            *reinterpret_cast<float4*>(mine_room + (((((c - c0) >> 2) + j) ^ (lane & (kUnits - 1))) << 4)) = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+                        for (int j = 0; j < 4; j++)
+                            *reinterpret_cast<float4*>(mine_room + (((((c - c0) >> 2) + j) ^ (lane & (kUnits - 1))) << 4)) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                     }
                 }
                 __syncwarp();
@@ -422,9 +410,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll 4
                 for (int i = 0; i < kUnits; i++) {
                     const int from = i * (32 / kUnits) + lane / kUnits;
-                    uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)dst, from));
+                    uint8_t* to = s_row[s][32 * quarter + from];
                     const uint4 x = *reinterpret_cast<const uint4*>(room + from * DP * 2 + ((unit ^ (from & (kUnits - 1))) << 4));
-                    if ((alive >> from & 1u) && byte < row_bytes) *reinterpret_cast<uint4*>(to + byte) = x;
+                    if (to && byte < row_bytes) *reinterpret_cast<uint4*>(to + byte) = x;
                 }
                 __syncwarp();
             }
@@ -442,7 +430,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             if (!dual && lane == 0) mbar_arrive(&o1_free);
             // the stream's other warps may still read where this one will put queries
             if (f32 && !mbar_wait_bounded(&o1_free, (uint32_t)(meets - 1) & 1u, err, 99)) { ok = false; break; }
-            items++;
+            taken++;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -453,14 +441,58 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
             uint8_t* room = keys ? sk : sv;
             PtItem it = {};
-            int nk = 0, items = 0;
+            int nk = 0, n_items = 0, u = u0;
             bool ok = true;
-            for (int u = u0; ok && u < u1; u += it.units) {
-                open(it, u, u != u0);
-                if (it.blocks <= 0) continue;
-                if (!f32 && keys) {
+            while (ok) {
+                if (keys) {
+                    // the CTA's next item that it has blocks of
+                    it.blocks = 0;
+                    while (u < u1 && it.blocks <= 0) {
+                        int at = 0;
+                        if (u == u0) {
+                            const int j = plan.find(u), per = (plan.cum[j + 1] - plan.cum[j]) / p.kv_heads;
+                            it.job = plan.known(p, j);
+                            at = u - plan.cum[j];
+                            it.head = at / per;
+                            at -= it.head * per;
+                            it.t0 = 0;
+                            for (int n = blocks_of(it.job, 0) + kPtExtra; at >= n; n = blocks_of(it.job, it.t0) + kPtExtra) {
+                                at -= n;
+                                it.t0 += item_tokens;
+                            }
+                        } else if (it.t0 + item_tokens < it.job.count) {
+                            it.t0 += item_tokens;
+                        } else {
+                            it.t0 = 0;
+                            if (++it.head == p.kv_heads) {
+                                it.job = plan.known(p, plan.find(u));
+                                it.head = 0;
+                            }
+                        }
+                        it.begin = u - at;
+                        it.end = it.begin + blocks_of(it.job, it.t0) + kPtExtra;
+                        it.tokens = min(item_tokens, it.job.count - it.t0);
+                        const int block = max(at - kPtExtra, 0);
+                        it.from = it.job.from + block * kPtKeys;
+                        it.blocks = min(it.end, u1) - it.begin - kPtExtra - block;          // (none: the next CTA has the first one)
+                        it.starts = block == 0;
+                        u = it.end;
+                    }
+                    const int slot = n_items % kPtItems;
+                    if (n_items >= kPtItems && !mbar_wait_bounded(&item_empty[slot], (uint32_t)(n_items / kPtItems - 1) & 1u, err, 101)) break;
+                    if (lane == 0) {
+                        items[slot] = it;
+                        mbar_arrive(&item_full[slot]);
+                    }
+                    __syncwarp();
+                    if (it.blocks <= 0) break;
+                } else if (!take(it, n_items, false)) {
+                    break;
+                }
+                // Queries, once the room of the last item's is free, which is while this one's first keys come.
+                auto queries = [&] {
                     const int tiles = is_dual(it) ? 2 : 1;
-                    if (items && !mbar_wait_bounded(&q_empty, (uint32_t)(items - 1) & 1u, err, 84)) break;
+                    if (n_items && !mbar_wait_bounded(&q_empty, (uint32_t)(n_items - 1) & 1u, err, 84)) return false;
                     if (lane == 0) {
                         mbar_expect_tx(&q_full, (uint32_t)(tiles * kHalves * tile_tokens * p.share * 128));
                         for (int s = 0; s < tiles; s++)
@@ -468,7 +500,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                             for (int h = 0; h < kHalves; h++)
                                 tma_rows_3d(sq + (s * kHalves + h) * kPtPiece, &qmap, 64 * h, it.head * p.share, it.job.first + it.t0 + s * tile_tokens, &q_full);
                     }
-                }
+                    return true;
+                };
                 // a lane per page (box) of a block
                 const int box_rows = p.page < kPtKeys ? p.page : kPtKeys, boxes = kPtKeys / box_rows;
                 const int* table = p.table + (size_t)it.job.seq * p.max_pages;
@@ -477,7 +510,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     return lane < boxes && key < it.job.to ? table[key >> p.log_page] : -2;
                 };
                 int entry = entry_of(0);
-                for (int b = 0; b < it.blocks; b++, nk++) {
+                for (int b = 0; b <= it.blocks; b++) {
+                    if (!f32 && keys && b == min(kDepth, it.blocks) && !(ok = queries())) break;
+                    if (b == it.blocks) break;
                     const int slot = nk % kDepth, now = entry;
                     if (b + 1 < it.blocks) entry = entry_of(b + 1);
                     const bool have = now >= 0 && now < p.n_pages;
@@ -498,8 +533,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     if (have)
                         for (int h = 0; h < (p.both ? 1 : kHalves); h++)
                             tma_page(smem_addr(room + (slot * kHalves + h) * kPtPiece + lane * box_rows * 128), map, 64 * h, row, it.head, now, smem_addr(&full[slot]));
+                    nk++;
                 }
-                items++;
+                n_items++;
             }
         } else {
             // ---------------- MMAs.  (What this thread computes between two products is a chain that nothing covers: addresses and descriptors are ready ahead.)
@@ -514,17 +550,15 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                b_vf = smem_addr(v_full), b_ve = smem_addr(v_empty);
                 const uint64_t kd0 = swizzled_desc(smem_addr(sk)), vd0 = swizzled_desc_mn(smem_addr(sv), kPtPiece);
                 PtItem it = {};
-                int items = 0;
+                int taken = 0;
                 uint32_t ks = 0, kp = 0, vs = 0, vp = 0;        // the next blocks of keys and values: slots and phases
                 uint32_t si = 0, pi = 0;                        // steps so far: scores, sums
                 bool ok = true;
-                for (int u = u0; ok && u < u1; u += it.units) {
-                    open(it, u, u != u0);
-                    if (it.blocks <= 0) continue;
+                while (ok && take(it, taken, true)) {
                     const bool dual = is_dual(it);
                     const int steps = dual ? 2 * it.blocks : it.blocks;
                     const uint64_t qd = swizzled_desc(smem_addr(sq + (dual ? s : 0) * kHalves * kPtPiece));
-                    if (!(ok = mbar_wait_bounded(&q_full, (uint32_t)items & 1u, err, 87))) break;
+                    if (!(ok = mbar_wait_bounded(&q_full, (uint32_t)taken & 1u, err, 87))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     // step t reads half `h` of a block; `first` and `last` of this stream's steps on it
                     auto scores = [&](int t) {
@@ -572,7 +606,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         pi++;
                         if (t + 2 < steps) ok = scores(t + 2);
                     }
-                    items++;
+                    taken++;
                 }
             }
         __syncwarp();
