@@ -97,10 +97,10 @@ struct PtItem {
 };
 constexpr int kPtItems = 4;             // a warp finds the items and puts them here; the others take them
 constexpr int kPtTakers = 1 + 2 + 8;
-// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as two blocks: it counts two units more than it has blocks, its first ones.  (Eight prompts' worth of 8000 tokens: none 692 us, one 595, two 555, three 555, eight 592.)
+// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as two blocks: it counts two units more than it has blocks, its first ones.  (One prompt of 8000 tokens, 32 heads on 8 of 128: none 692 us, one 595, two 555, three 555, eight 592.)
 constexpr int kPtExtra = 2;
 
-template <typename A, typename K, int DP>
+template <typename A, typename K, int DP, bool kCap>
 __global__ void __launch_bounds__(kPtThreads, 1)
 k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedArgs p, int* err)
 {
@@ -226,10 +226,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 if (!mbar_wait_bounded(&q_full, (uint32_t)taken & 1u, err, 91)) { ok = false; break; }
                 f *= s_factor[r];
             }
-            const float sign = f < 0.0f ? -1.0f : 1.0f;
-            f = fabsf(f);
-            const bool plain = p.cap <= 0.0f && __all_sync(0xFFFFFFFFu, sign > 0.0f);
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
+            const bool negative = p.scale < 0.0f;
             float top = -INFINITY, sum = 0.0f;          // in units of log2
             for (int t = 0; t < n_steps; t++, steps++) {
                 const int b = dual ? t >> 1 : t, half = dual ? t & 1 : s, key = it.from + b * kPtKeys + half * kPtStep;
@@ -241,17 +239,14 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 tmem_ld_32(ts + 32, v + 32);
                 tmem_loaded();
                 const unsigned missing = s_missing[(nk + b) & 7] >> (8 * half) & 0xFFu;
-                const bool edge = key + kPtStep > least || missing;
+                // (where the scale is negative the largest score is the least product)
+                const bool edge = key + kPtStep > least || missing || (!kCap && negative);
                 float ff = f;
-                if (plain) {
-                } else if (p.cap > 0.0f) {
-                    const float in = sign * f * 0.69314718055994531f;
+                if (kCap) {
+                    const float in = f * 0.69314718055994531f;
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[j] = capped<f32>(v[j] * in, p.cap) * 1.44269504088896341f;
                     ff = 1.0f;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 64; j++) v[j] *= sign;
                 }
                 if (edge) {
 #pragma unroll
@@ -489,7 +484,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 } else if (!take(it, n_items, false)) {
                     break;
                 }
-                // Queries, once the room of the last item's is free, which is while this one's first keys come.
+                // Queries, once the room of the last item's is free, which is while this one's first keys come.  (The first item's need not wait for any, and the first products wait for them.)
                 auto queries = [&] {
                     const int tiles = is_dual(it) ? 2 : 1;
                     if (n_items && !mbar_wait_bounded(&q_empty, (uint32_t)(n_items - 1) & 1u, err, 84)) return false;
@@ -511,7 +506,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 };
                 int entry = entry_of(0);
                 for (int b = 0; b <= it.blocks; b++) {
-                    if (!f32 && keys && b == min(kDepth, it.blocks) && !(ok = queries())) break;
+                    if (!f32 && keys && b == (n_items ? min(kDepth, it.blocks) : 0) && !(ok = queries())) break;
                     if (b == it.blocks) break;
                     const int slot = nk % kDepth, now = entry;
                     if (b + 1 < it.blocks) entry = entry_of(b + 1);
@@ -621,7 +616,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     }
 }
 
-template <typename A, typename K, int DP>
+template <typename A, typename K, int DP, bool kCap>
 static int launch_tile(PagedArgs a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
 {
     CUtensorMap qmap, kmap, vmap;
@@ -633,17 +628,22 @@ static int launch_tile(PagedArgs a, const bpdq_paged_kv& kv, int ctas, cudaStrea
         const int tokens = kPtRows / a.share;
         if ((rc = bf16_map(&qmap, a.q, a.dim, a.heads, a.dim, a.share, a.n_tokens, a.ld_q, tokens))) return rc;
     }
-    if ((rc = allow_smem<k_paged_tile<A, K, DP>>(221 * 1024))) return rc;
+    if ((rc = allow_smem<k_paged_tile<A, K, DP, kCap>>(221 * 1024))) return rc;
     const size_t smem = 1024 + PtShape<DP>::end + PagedPlan::size(a);
-    return launch_ordered(k_paged_tile<A, K, DP>, dim3((unsigned)ctas), kPtThreads, smem, s, qmap, kmap, vmap, a, device_error_flag());
+    return launch_ordered(k_paged_tile<A, K, DP, kCap>, dim3((unsigned)ctas), kPtThreads, smem, s, qmap, kmap, vmap, a, device_error_flag());
+}
+
+template <typename A, typename K>
+static int launch_kind(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
+{
+    if (a.dim > 64) return a.cap > 0.0f ? launch_tile<A, K, 128, true>(a, kv, ctas, s) : launch_tile<A, K, 128, false>(a, kv, ctas, s);
+    return a.cap > 0.0f ? launch_tile<A, K, 64, true>(a, kv, ctas, s) : launch_tile<A, K, 64, false>(a, kv, ctas, s);
 }
 
 int paged_tile(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
 {
-    const bool wide = a.dim > 64;
-    if (kv.act_type == BPDQ_TYPE_F32) return wide ? launch_tile<float, __half, 128>(a, kv, ctas, s) : launch_tile<float, __half, 64>(a, kv, ctas, s);
-    if (kv.kv_type == BPDQ_TYPE_F16) return wide ? launch_tile<__half, __half, 128>(a, kv, ctas, s) : launch_tile<__half, __half, 64>(a, kv, ctas, s);
-    return wide ? launch_tile<bf16, bf16, 128>(a, kv, ctas, s) : launch_tile<bf16, bf16, 64>(a, kv, ctas, s);
+    if (kv.act_type == BPDQ_TYPE_F32) return launch_kind<float, __half>(a, kv, ctas, s);
+    return kv.kv_type == BPDQ_TYPE_F16 ? launch_kind<__half, __half>(a, kv, ctas, s) : launch_kind<bf16, bf16>(a, kv, ctas, s);
 }
 
 }  // namespace bpdq
