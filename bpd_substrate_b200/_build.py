@@ -14,7 +14,7 @@ SOURCES = ["runtime.cu", "dequant_q4k.cu", "gemv_q4k.cu", "gemv_batch.cu", "gemv
 # The sources some model families need: a process that only serves one of those (bin/trace_run in a fresh checkout)
 # compiles and loads these as a library of their own when the whole one has not been built.
 PARTS = {"hybrid": ["runtime.cu", "decode_ops.cu", "linear.cu", "decayed_scan.cu", "latent_attention.cu", "delta_rule.cu", "grouped_attention.cu", "prompt_attention.cu",
-                    "residual_streams.cu", "hybrid_forward.cu"]}
+                    "residual_streams.cu", "hybrid_forward.cu", "sample.cu"]}
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",

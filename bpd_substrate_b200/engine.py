@@ -1,15 +1,16 @@
 """Generation: sequences of a model in slots, prompts in portions, one token per step after that.
 
 A model brings ``state_parts()``, ``capacity``, ``vocab``, ``stream``, ``lib`` and
-``step(seq, tokens, want, logits)``, ``portion`` if a step takes no more tokens than that, and ``forget(base, nbytes)`` if it keeps
+``step(seq, tokens, want, logits)``, ``sample(seq, tokens, rule, u)`` for requests that are not greedy, ``portion`` if a step takes no more tokens than that, and ``forget(base, nbytes)`` if it keeps
 anything by a state's address; the engine is the same for every family.  A step runs one sequence:
 the next portion of its prompt or its last token.  Live requests take turns.
 """
 from collections import deque
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import numpy as np
 
+from .sampling import Sampling
 from .sequences import SequenceSlots
 
 
@@ -18,9 +19,11 @@ class Request:
     prompt: list
     max_new_tokens: int
     stop: frozenset = frozenset()
+    sampling: Sampling = None     # None: greedy
     output: list = field(default_factory=list)
     fed: int = 0              # prompt tokens that have been run
     key: object = None
+    numbers: object = None    # of its sampling
 
 
 class Engine:
@@ -68,17 +71,27 @@ class Engine:
         if r.fed < len(r.prompt):
             part = r.prompt[r.fed:r.fed + self.portion]
             last = r.fed + len(part) == len(r.prompt)
-            _, ids = self.feed(r.key, part, [len(part) - 1] if last else [], logits=False)
-            r.fed += len(part)
             if not last:
+                self.feed(r.key, part, [], logits=False)
+                r.fed += len(part)
                 return False
+            r.output.append(self._next(r, part))
+            r.fed += len(part)
         else:
-            _, ids = self.feed(r.key, r.output[-1:], [0], logits=False)
-        r.output.append(int(ids[0]))
+            r.output.append(self._next(r, r.output[-1:]))
         return len(r.output) >= r.max_new_tokens or r.output[-1] in r.stop
 
+    def _next(self, r, tokens):
+        """Runs the request's next tokens; returns the one that follows them."""
+        if r.sampling is None:
+            return int(self.feed(r.key, tokens, [len(tokens) - 1], logits=False)[1][0])
+        picked = self.model.sample(self.live[r.key], np.asarray(tokens, np.int32), r.sampling, float(r.numbers.random(dtype=np.float32)))
+        if picked < 0:
+            raise ValueError("no token is left to choose: not one logit is above -inf")
+        return picked
+
     def run(self, requests):
-        """Greedy generation of all requests, oldest first into free slots; fills their `output`."""
+        """Generation of all requests, oldest first into free slots; fills their `output`."""
         for i, r in enumerate(requests):
             r.key = ("request", i)
             if not len(r.prompt) or r.max_new_tokens < 1:
@@ -99,10 +112,12 @@ class Engine:
 
     def _start(self, r):
         self.live[r.key] = self.slots.acquire()
+        r.numbers = r.sampling.numbers() if r.sampling else None
 
-    def generate(self, prompts, max_new_tokens, stop=()):
-        """Greedy continuation of every prompt: a list of token lists."""
-        return [r.output for r in self.run([Request(list(p), max_new_tokens, frozenset(stop)) for p in prompts])]
+    def generate(self, prompts, max_new_tokens, stop=(), sampling=None):
+        """A continuation of every prompt, greedy or by `sampling` (prompt i with its seed + i): a list of token lists."""
+        rules = [replace(sampling, seed=sampling.seed + i) if sampling else None for i in range(len(prompts))]
+        return [r.output for r in self.run([Request(list(p), max_new_tokens, frozenset(stop), s) for p, s in zip(prompts, rules)])]
 
     def close(self):
         block, nbytes = self.slots.block, self.slots.nbytes

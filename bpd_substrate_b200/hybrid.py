@@ -14,6 +14,7 @@ import numpy as np
 
 from . import capi
 from .safetensors_load import SafetensorsFile, bf16_to_f32
+from .sampling import TokenSampler
 from .sequences import StatePart, lay_out
 
 MAX_TOKENS = 65535      # of one step
@@ -351,7 +352,7 @@ class DeviceHybrid:
         self.spec, self.vocab, self.dtype, self.capacity, self.use_graph = spec, spec.vocab, dtype, capacity, use_graph
         self._own_stream = stream is None
         self.stream = lib.bpdq_stream_create() if stream is None else stream
-        self._allocs, self.weight_bytes = [], 0
+        self._allocs, self.weight_bytes, self._sampler = [], 0, None
         spec.read_shapes(get.shape)
         self.parts = spec.state_parts(dtype == "bfloat16")
         offsets, rows = lay_out(self.parts, capacity).offsets, {p.name: p.count(capacity) for p in self.parts}
@@ -448,6 +449,13 @@ class DeviceHybrid:
         seq.length += tokens.size
         return out, picked
 
+    def sample(self, seq, tokens, rule, u):
+        """Runs the tokens; returns the one that follows them by the rule (sampling.Sampling) and the random number u.  The logits stay on the device."""
+        if self._sampler is None:
+            self._sampler = TokenSampler(self.lib, self.stream)
+        self.launch(seq, tokens, [len(tokens) - 1])
+        return self._sampler.pick(self.lib.bpdq_hybrid_logits(self.plan), self.vocab, rule, u)
+
     def residuals(self, seq, tokens):
         """The residual stream after every layer, [layers, tokens, width]."""
         n, L = len(tokens), len(self.spec.layers)
@@ -465,6 +473,9 @@ class DeviceHybrid:
         self.lib.bpdq_stream_sync(self.stream)
         self.lib.bpdq_hybrid_destroy(self.plan)
         self.plan = None
+        if self._sampler:
+            self._sampler.close()
+            self._sampler = None
         for p in self._allocs:
             self.lib.bpdq_free(p)
         self._allocs = []

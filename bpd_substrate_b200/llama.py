@@ -12,6 +12,7 @@ import ctypes as C
 import numpy as np
 
 from . import capi, synth
+from .sampling import TokenSampler
 from .sequences import SequenceSlots, StatePart, lay_out
 
 LAYER_FIELDS = ("attn_norm_w", "w_q", "w_k", "w_v", "w_o", "ffn_norm_w", "w_gate", "w_up", "w_down")
@@ -126,7 +127,7 @@ class DeviceLlama:
         self.vocab, self.capacity = self.cfg.vocab_size, self.cfg.max_seq_len
         self.kv_bytes = model.kv_cache()[0].nbytes
         self._offsets = lay_out(self.state_parts(), self.capacity).offsets
-        self._slots = self._own = None
+        self._slots = self._own = self._sampler = None
         self.stream = lib.bpdq_stream_create()
         capi.check(lib.bpdq_last_status(), "DeviceLlama setup")
 
@@ -183,6 +184,17 @@ class DeviceLlama:
         want = list(want)
         return (out[want] if logits else None), picked[want]
 
+    def sample(self, seq, tokens, rule, u):
+        """Runs the next tokens of `seq`; returns the one that follows them by the rule (sampling.Sampling) and the random number u."""
+        if self._sampler is None:
+            self._sampler = TokenSampler(self.lib, self.stream)
+        pos = np.arange(seq.length, seq.length + len(tokens), dtype=np.int32)
+        last = 4 * self.vocab * (len(tokens) - 1)
+        picked = self._run(tokens, pos, seq.length, seq.base + self._offsets["k"], seq.base + self._offsets["v"],
+                           lambda logits: self._sampler.pick(logits + last, self.vocab, rule, u))
+        seq.length += len(tokens)
+        return picked
+
     def reset_cache(self):
         capi.check(self.lib.bpdq_memset_async(self.d_k, 0, self.kv_bytes, self.stream))
         capi.check(self.lib.bpdq_memset_async(self.d_v, 0, self.kv_bytes, self.stream))
@@ -191,7 +203,8 @@ class DeviceLlama:
         """Runs the tokens through all layers; returns (logits [n, vocab], argmax tokens [n])."""
         return self._run(token_ids, pos_ids, kv_pos, self.d_k, self.d_v)
 
-    def _run(self, token_ids, pos_ids, kv_pos, d_k, d_v):
+    def _run(self, token_ids, pos_ids, kv_pos, d_k, d_v, pick=None):
+        """(logits, argmax tokens) on the host, or what `pick` makes of the logits' device address."""
         lib = self.lib
         token_ids = np.ascontiguousarray(token_ids, np.int32)
         pos_ids = np.ascontiguousarray(pos_ids, np.int32)
@@ -205,6 +218,8 @@ class DeviceLlama:
             capi.check(lib.bpd_llama_forward_tiles_cuda(d_tok, n, C.byref(self.weights), tiles, C.byref(self.cfg), d_pos, kv_pos,
                                                         d_k, d_v, d_logits, d_out, self.stream),
                        "bpd_llama_forward_tiles_cuda")
+            if pick is not None:
+                return pick(d_logits)
             capi.check(lib.bpdq_stream_sync(self.stream))
             logits = np.empty((n, self.cfg.vocab_size), np.float32)
             tokens = np.empty(n, np.int64)
@@ -228,6 +243,9 @@ class DeviceLlama:
         for p in self._allocs:
             self.lib.bpdq_free(p)
         self._allocs = []
+        if self._sampler:
+            self._sampler.close()
+            self._sampler = None
         if self._slots is not None:
             self._slots.close()
         self.lib.bpdq_stream_destroy(self.stream)
