@@ -407,6 +407,48 @@ def test_cache_beyond_four_gigabytes(lib):
         assert ((o[b].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 1e-4) * size).all()
 
 
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("H,G,D", [(34, 2, 64), (32, 1, 128), (128, 1, 128), (128, 1, 64), (200, 2, 40)])
+def test_many_heads_on_a_key_head(lib, act, kv, H, G, D):
+    """More rows per token than the kernel for few takes, up to a whole tile; shares that leave a tile's last rows empty."""
+    attention_case(lib, H, G, D, act, kv, 16, [0, 5, 300, 64], [1] * 4, seed=H)
+    attention_case(lib, H, G, D, act, kv, 16, [0, 5, 300, 64], [9, 1, 2, 30], seed=H, pad=1)
+    attention_case(lib, H, G, D, act, kv, 16, [200, 200, 230], [1, 2, 1], shared=[(0, 3, 12)], seed=H)
+
+
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("H,G,new", [(16, 4, [4] * 7), (16, 4, [4, 3, 2, 4, 1, 0, 4]), (16, 2, [2] * 7), (16, 2, [2, 1, 2, 2, 1, 1, 2]), (4, 4, [16, 9, 12, 10, 16, 11, 13]), (6, 2, [5, 3, 4, 5, 4, 5, 3])])
+def test_a_few_tokens_each(lib, act, kv, H, G, new):
+    """Guessed tokens checked in one step: nine to sixteen rows of a sequence."""
+    held = [0, 1, 15, 400, 2000, 33, 127]
+    attention_case(lib, H, G, 128, act, kv, 16, held, new, seed=H, ragged=True)
+    attention_case(lib, H, G, 64, act, kv, 32, held, new, seed=H, ragged=True, cap=15.0, pad=3)
+    attention_case(lib, H, G, 128, act, kv, 16, [500] * 7, new, seed=H, ragged=True, shared=[(0, 3, 20), (3, 7, 31)])
+
+
+@pytest.mark.parametrize("page", [8, 32, 64, 128, 256])
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_page_sizes(lib, act, kv, page):
+    """Pages smaller and larger than a block of keys, shared ones among them, which a block may begin inside."""
+    n = 512 // page
+    for H, G, D in ((8, 2, 128), (4, 1, 72)):
+        attention_case(lib, H, G, D, act, kv, page, [512 + 9, 512, 700, 600], [1] * 4, shared=[(0, 4, n)], seed=page)
+        attention_case(lib, H, G, D, act, kv, page, [512 + 9, 512, 700, 600, 0], [1, 70, 300, 2, 260], shared=[(0, 4, n)], seed=page)
+
+
+@pytest.mark.parametrize("batch,sets", [(1280, 0), (1000, 280), (1278, 2)])
+def test_as_many_sequences_as_there_may_be(lib, batch, sets):
+    """With one token each, and with a long prompt among them."""
+    gen = torch.Generator().manual_seed(batch)
+    held = (torch.randint(0, 60, (batch,), generator=gen) + 16).tolist()
+    shared = [(batch * i // sets, batch * (i + 1) // sets, 1) for i in range(sets)]
+    attention_case(lib, 4, 2, 64, "bf16", "bf16", 16, held, [1] * batch, shared=shared)
+    new = [1] * batch
+    new[batch // 3] = 200
+    new[batch // 2] = 0
+    attention_case(lib, 4, 2, 64, "bf16", "bf16", 16, held, new, shared=shared)
+
+
 # ---- workspaces, streams, recordings
 
 @pytest.mark.parametrize("new", [[1] * 6, [1, 40, 1, 300, 2, 1]])
@@ -457,6 +499,40 @@ def test_own_scratch_and_recordings(lib, new):
     lib.bpdq_clear_status()
     lib.bpdq_graph_destroy(rec)
     lib.bpdq_stream_destroy(s)
+
+
+@pytest.mark.parametrize("new", [[1] * 5, [1, 150, 1, 33, 4]])
+def test_two_at_once(lib, new):
+    """Two streams' recordings, each with its scratch, side by side and again and again, give what each gives alone."""
+    runs = []
+    for i in range(2):
+        c = Cache(8, 2, 128, "bf16", "bf16", 16, [800 + 300 * i, 0, 777, 63, 2000], new, 20 + i)
+        c.fill()
+        q = torch.randn(c.tokens, 1024, generator=c.gen).bfloat16().cuda()
+        desc = c.upload()
+        size = lib.bpdq_paged_attention_workspace_bytes(desc, c.tokens, None)
+        ws, o = torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255), torch.full_like(q, 9.0)
+        want = torch.empty_like(q)
+        torch.cuda.synchronize()
+        done(lib, lib.bpd_paged_attention_cuda(desc, q.data_ptr(), 1024, want.data_ptr(), 1024, c.tokens, 0.1, 0.0, None, None))
+        stream = lib.bpdq_stream_create()
+        assert lib.bpdq_graph_begin(stream) == 0
+        for _ in range(5):
+            assert lib.bpd_paged_attention_ws_cuda(desc, q.data_ptr(), 1024, o.data_ptr(), 1024, c.tokens, 0.1, 0.0, None, ws.data_ptr(), size, stream) == 0
+        rec = lib.bpdq_graph_end(stream)
+        assert rec
+        runs.append((c, q, desc, ws, o, want, stream, rec))
+    for _ in range(20):
+        for *_, stream, rec in runs:
+            assert lib.bpdq_graph_launch(rec, stream) == 0
+    for c, q, desc, ws, o, want, stream, rec in runs:
+        assert lib.bpdq_stream_sync(stream) == 0
+    torch.cuda.synchronize()
+    assert lib.bpdq_last_status() == 0
+    for c, q, desc, ws, o, want, stream, rec in runs:
+        assert torch.equal(o, want)
+        lib.bpdq_graph_destroy(rec)
+        lib.bpdq_stream_destroy(stream)
 
 
 # ---- together
