@@ -102,11 +102,11 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedArgs p)
                     sum = fmaf(w, s_ml[i].y, sum);
                     o = fmaf(w, s_o[kFew ? i : 0][d], o);
                 }
-                out[d] = ActOf<A>::put(sum > 0.0f ? o / sum : 0.0f);
+                out[d] = ActOf<A>::put(sum != 0.0f ? o / sum : 0.0f);
             }
             continue;
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
         for (int c = 0; c < kUnits; c++)
             if (32 * c + 4 * l8 < p.dim) {
@@ -146,6 +146,7 @@ static size_t carve(PagedArgs& a, uint8_t* base, int ctas, bool tiles)
     if (tiles) {
         take(a.tile_o, (size_t)2 * ctas * kTileRows * pad);
         take(a.tile_ml, (size_t)2 * ctas * kTileRows);
+        if (a.f32) take(a.tile_sums, (size_t)ctas * kTileRows * pad);
     }
     if (a.groups) {
         take(a.prefix, rows);
@@ -172,7 +173,7 @@ static PagedArgs arguments(const bpdq_paged_kv& kv, int n_tokens, const bpdq_pag
     p.n_tokens = n_tokens; p.batch = kv.batch; p.heads = kv.heads; p.kv_heads = kv.kv_heads; p.share = kv.heads / kv.kv_heads; p.dim = kv.dim;
     p.page = kv.page; p.max_pages = kv.max_pages; p.n_pages = kv.n_pages; p.page_stride = paged_stride(kv);
     while ((1 << p.log_page) < p.page) p.log_page++;
-    p.seq_start = kv.seq_start; p.length = kv.length; p.table = kv.page_table;
+    p.seq_start = kv.seq_start; p.length = kv.length; p.table = kv.page_table; p.f32 = kv.act_type == BPDQ_TYPE_F32;
     if (groups && groups->n) { p.groups = groups->n; p.group_start = groups->start; p.group_pages = groups->pages; }
     return p;
 }

@@ -20,6 +20,7 @@ struct PagedArgs {
     float scale, cap;
     int split_rows;             // jobs of up to so many rows are k_paged_split's, the others k_paged_tile's
     int both;                   // this launch's requests bring both halves of 128 dimensions
+    int f32;                    // activations
     int mark;                   // this launch says which tokens belong to no sequence
     // scratch
     int4* own;                  // [tokens][heads]: what k_paged_join finds of a row's own positions
@@ -28,6 +29,7 @@ struct PagedArgs {
     float2 *own_ml, *prefix_ml; // their maxima (in units of log2) and sums
     float *split_o, *tile_o;    // parts of items that several CTAs share: [2 * CTA + which][rows][dim_pad]
     float2 *split_ml, *tile_ml;
+    float* tile_sums;           // k_paged_tile of fp32: what a stream has put aside, [2 * CTA + stream][dim_pad / 4][rows of a stream][4]
     float* head_o;              // k_paged_split: a warp's first part, when it has two
     float2* head_ml;
 };

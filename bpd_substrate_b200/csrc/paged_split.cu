@@ -352,7 +352,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const size_t row = (size_t)tok * p.heads + h;
             float* dst = nullptr;
             if (all && !it.job.joined) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
                 A* o = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim;
 #pragma unroll
                 for (int i = 0; i < kOut; i++)
@@ -437,7 +437,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         const int t = r / p.share, tok = item.first + t, h = item.head * p.share + r - t * p.share;
         const size_t row = (size_t)tok * p.heads + h;
         if (all && !item.joined) {
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
             A* out_row = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim + 4 * l8;
 #pragma unroll
             for (int c = 0; c < kHalves * 2; c++)

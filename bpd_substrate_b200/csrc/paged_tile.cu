@@ -23,6 +23,9 @@ namespace bpdq {
 constexpr int kPtRows = 128, kPtKeys = 128, kPtStep = 64, kPtPiece = 128 * 64 * 2;     // rows of a tile, keys of a block and of a step, bytes of 128 rows x 64 columns
 constexpr int kPtWarps = 8, kPtThreads = 32 * (4 + kPtWarps);          // three groups of four warps, which have registers of their own size
 constexpr float kPtGrowth = 8.0f;
+// The tensor pipe cuts off what does not fit fp32 of each of its sums, always toward zero: 6000 keys in one go are 4e-6 short.  With fp32 activations a stream
+// puts its sums aside every so many steps, added to the last ones as fp32 numbers round, and begins anew.
+constexpr int kPtFold = 8;
 
 template <int DP> struct PtShape {
     static constexpr int halves = DP / 64, depth = DP == 64 ? 4 : 2;        // blocks of keys (and of values) in shared memory
@@ -76,7 +79,8 @@ __device__ __forceinline__ float2 add_two(float2 a, float2 b)
 // keeps 8 to 11 bits).  0 from 2^-127 down.
 __device__ __forceinline__ float2 ex2_two(float2 x)
 {
-    x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.0f));        // (a NaN stays one)
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.0f));
     const float2 shift = make_float2(12582912.0f, 12582912.0f), back = make_float2(-12582912.0f, -12582912.0f), minus = make_float2(-1.0f, -1.0f);
     const float2 k = add_two(x, shift), f = fma_two(add_two(k, back), minus, x);
     float2 p = make_float2(9.5605102e-3f, 9.5605102e-3f);
@@ -97,7 +101,8 @@ struct PtItem {
 };
 constexpr int kPtItems = 4;             // a warp finds the items and puts them here; the others take them
 constexpr int kPtTakers = 1 + 2 + 8;
-// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as two blocks: it counts two units more than it has blocks, its first ones.  (One prompt of 8000 tokens, 32 heads on 8 of 128: none 692 us, one 595, two 555, three 555, eight 592.)
+// An item's beginning and end (queries, a pipe that runs empty, results) take about as long as two blocks: it counts two units more than it has blocks, its first ones.
+// (One prompt of 8000 tokens, 32 heads on 8 of 128: none 692 us, one 595, two 555, three 555, eight 592.)
 constexpr int kPtExtra = 2;
 
 template <typename A, typename K, int DP, bool kCap>
@@ -115,7 +120,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     __shared__ unsigned short s_missing[8];             // of a block: groups of eight keys without a page; softmax is two blocks behind the copies' kDepth at most
     __shared__ float2 s_ml[kPtRows];
     __shared__ uint8_t* s_row[2][kPtRows];              // where rows go; null: nowhere
-    __shared__ float s_factor[kPtRows];
+    __shared__ float s_factor[kPtRows], s_aside[kPtRows];
     uint8_t* base = raw + (((smem_addr(raw) + 1023) & ~1023u) - smem_addr(raw));
     uint8_t *sq = base + Shape::q, *sk = base + Shape::k, *sv = base + Shape::v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -229,6 +234,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             const bool negative = p.scale < 0.0f;
             float top = -INFINITY, sum = 0.0f;          // in units of log2
+            float aside_top = -INFINITY;                // of the sums put aside
+            float4* aside = f32 ? reinterpret_cast<float4*>(p.tile_sums) + ((size_t)(2 * cta + s) * (DP / 4)) * kPtRows + r : nullptr;
             for (int t = 0; t < n_steps; t++, steps++) {
                 const int b = dual ? t >> 1 : t, half = dual ? t & 1 : s, key = it.from + b * kPtKeys + half * kPtStep;
                 const uint32_t ts = tmem + lanes + 128 * s + 64 * (steps & 1);
@@ -261,7 +268,28 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 }
                 const float now = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * ff;
                 const bool grown = now > top + kPtGrowth;
-                if (t > 0 && __any_sync(0xFFFFFFFFu, grown)) {
+                const bool fold = f32 && t > 0 && t % kPtFold == 0;
+                if (fold) {
+                    if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 93)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const float down = aside_top == -INFINITY ? 0.0f : ex2(aside_top - top);
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 16) {
+                        int ov[16];
+                        tmem_ld(to_ + 128 * s + c, ov);
+                        float4 x[4] = {};
+                        if (t > kPtFold)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) x[j] = __ldcg(aside + (c / 4 + j) * kPtRows);
+                        tmem_loaded();
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            __stcg(aside + (c / 4 + j) * kPtRows, make_float4(fmaf(x[j].x, down, __int_as_float(ov[4 * j])), fmaf(x[j].y, down, __int_as_float(ov[4 * j + 1])),
+                                                                              fmaf(x[j].z, down, __int_as_float(ov[4 * j + 2])), fmaf(x[j].w, down, __int_as_float(ov[4 * j + 3]))));
+                    }
+                    aside_top = top;
+                    if (grown) sum *= ex2(top - now);
+                } else if (t > 0 && __any_sync(0xFFFFFFFFu, grown)) {
                     if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 93)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const float down = grown ? ex2(top - now) : 1.0f;
@@ -331,9 +359,12 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             // ---- the item's sums, or this CTA's part of them
             if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 95)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float w0 = 1.0f, w1 = 0.0f;
+            float w0 = 1.0f, w1 = 0.0f, a0 = 0.0f, a1 = 0.0f;       // what the streams' sums count, and those put aside
             if (!dual) {
-                if (s == 1) s_ml[r] = make_float2(top, sum);
+                if (s == 1) {
+                    s_ml[r] = make_float2(top, sum);
+                    s_aside[r] = aside_top;
+                }
                 __syncwarp();
                 if (s == 1) {
                     if (lane == 0) mbar_arrive(&ml_ready);
@@ -352,6 +383,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     const float most = fmaxf(top, odd.x), zero = most == -INFINITY ? 0.0f : most;
                     w0 = ex2(top - zero);
                     w1 = ex2(odd.x - zero);
+                    a0 = ex2(aside_top - zero);
+                    a1 = ex2(s_aside[r] - zero);
                     sum = w0 * sum + w1 * odd.y;
                     top = most;
                 }
@@ -362,9 +395,11 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             const size_t at = all ? row : (size_t)(2 * cta + starts) * kTileRows + in_part;
             const bool direct = all && !it.job.joined;
             if (direct) {
-                const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
                 w0 *= inv;
                 w1 *= inv;
+                a0 *= inv;
+                a1 *= inv;
             }
             // Rows pass through the room of the item's queries, of which a warp has an eighth, so that whole lines of them are stored: DP * 2 bytes of a row at a time, 16-byte
             // units turned by the row.
@@ -388,6 +423,16 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     for (int j = 0; j < 16; j++) {
                         o[j] = __int_as_float(x[j]) * w0;
                         if (!dual) o[j] = fmaf(__int_as_float(y[j]), w1, o[j]);
+                    }
+                    if (f32 && n_steps > kPtFold) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float4 u = __ldcg(aside + (c / 4 + j) * kPtRows), v = __ldcg(aside + (DP / 4 + c / 4 + j) * kPtRows);
+                            o[4 * j] += fmaf(u.x, a0, v.x * a1);
+                            o[4 * j + 1] += fmaf(u.y, a0, v.y * a1);
+                            o[4 * j + 2] += fmaf(u.z, a0, v.z * a1);
+                            o[4 * j + 3] += fmaf(u.w, a0, v.w * a1);
+                        }
                     }
                     if (narrow) {
 #pragma unroll
@@ -563,13 +608,13 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         const uint64_t kd = kd0 + ks * block + h * half_block;
                         const uint32_t to = scores_at + 64 * (si & 1);
 #pragma unroll
-                        for (int part = 0; part < (f32 ? 2 : 1); part++)
+                        for (int part = f32 ? 1 : 0; part >= 0; part--)         // (the small parts first: the sum is cut off at its own last bit)
 #pragma unroll
                             for (int c = 0; c < kHalves; c++)
 #pragma unroll
                                 for (int k = 0; k < 4; k++)
                                     umma_bf16_ss(to, qd + (uint64_t)((part * kHalves + c) * (kPtPiece >> 4) + 2 * k), kd + (uint64_t)(c * (kPtPiece >> 4) + 2 * k), idesc_s,
-                                                 part | c | k ? 1u : 0u);
+                                                 (f32 && part == 0) | c | k ? 1u : 0u);
                         umma_commit_at(b_s + 8 * (si & 1));
                         if (last) {
                             umma_commit_at(b_ke + 8 * ks);
@@ -590,7 +635,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         const uint32_t w = scores_at + 64 * (pi & 1);
 #pragma unroll
                         for (int k = 0; k < kPtStep / 16; k++) {
-                            if (f32) umma_bf16_ts(o, w + 32 + 8 * k, vd + (uint64_t)(k * 128), idesc_o, t | k ? 1u : 0u);
+                            if (f32) umma_bf16_ts(o, w + 32 + 8 * k, vd + (uint64_t)(k * 128), idesc_o, t % kPtFold | k ? 1u : 0u);
                             umma_bf16_ts(o, w + 8 * k, vd + (uint64_t)(k * 128), idesc_o, f32 || (t | k) ? 1u : 0u);
                         }
                         umma_commit_at(b_o + 8 * (pi & 1));

@@ -622,7 +622,8 @@ typedef struct {
     const int32_t *start, *pages;
 } bpdq_paged_groups;
 /* o[t][h] = sum_j softmax_j(s_j) v_j over the positions up to the token's own, s = scale q.k, with cap > 0 then cap tanh(s / cap).  The tokens' own keys and values are in the cache
- * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q.  fp32 activations keep fp32 sums' accuracy (queries and weights enter the tensor
+ * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q.  What lies in a page's other places is never looked at; the values
+ * at a sequence's positions, the call's new ones too, have to be finite (those behind a token meet weights of 0).  fp32 activations keep fp32 sums' accuracy (queries and weights enter the tensor
  * cores as two fp16 numbers each).  groups NULL: none.  A sequence's sums are split over the GPU by a rule on all lengths of the call: its last bits may depend
  * on what else is in the batch.  Up to 128 query heads per key head, 1280 sequences and
  * groups together; batch * kv_heads * max_pages * page up to 2^33.  Scratch: see "scratch memory" above; its size does not depend on lengths. */

@@ -366,6 +366,31 @@ def test_bad_pages_and_lengths(lib, new):
     assert miss.max() <= 0
 
 
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (4, 2, 64)])
+@pytest.mark.parametrize("held,new", [([100, 100, 30], [1, 1, 1]), ([100, 60, 30], [90, 3, 200])])
+def test_a_key_without_a_number(lib, act, kv, H, G, D, held, new):
+    """A NaN among the keys shows in the rows that see it, wherever it lies in a block, and in no others."""
+    for place in (70, 71, 72, 73, 74, 75, 76, 77, 100):
+        c = Cache(H, G, D, act, kv, 16, held, new, place)
+        c.fill()
+        clean = c.k.clone()
+        c.k[c.table[0, place // 16].long(), 1, place % 16, 5] = float("nan")
+        q = torch.randn(c.tokens, H * D, generator=c.gen).to(TYPES[act][0])
+        desc, d, o = c.upload(), q.cuda(), torch.full((c.tokens, H * D), 9.0, dtype=TYPES[act][0], device="cuda")
+        torch.cuda.synchronize()
+        done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), H * D, o.data_ptr(), H * D, c.tokens, 0.1, 0.0, None, None))
+        c.k.copy_(clean)
+        want, size, top = attention_oracle(c, q, 0.1, 0.0)
+        got = o.double().view(c.tokens, H, D)
+        sees = torch.zeros(c.tokens, H, dtype=torch.bool)
+        for t in range(new[0]):
+            sees[t, H // G:] = held[0] + t >= place
+        sees = sees.cuda()
+        assert torch.isnan(got[sees]).all()
+        assert ((got - want).abs() <= tolerance(c, want, size, top, 0.0))[~sees].all()
+
+
 def test_a_sequence_without_a_page_is_zero(lib):
     c = Cache(4, 2, 64, "bf16", "bf16", 16, [20, 20], [1, 1], 3)
     c.fill()
