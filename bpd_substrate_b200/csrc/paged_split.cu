@@ -209,7 +209,23 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     };
 
     // ---- sums
-    float out[MT][kOut][4], top[MT], sum[MT];
+    // (The tensor pipe cuts off what does not fit fp32 of each of its sums, always toward zero: with fp32 activations a tile's products start from 0 and are added here.)
+    constexpr int kSums = f32 ? 2 : 4;
+    float out[MT][kOut][kSums], top[MT], sum[MT];
+    auto result = [&](int m, int i, int c) {
+        if constexpr (f32) return out[m][i][c];
+        else return out[m][i][c] + out[m][i][c + 2];
+    };
+    auto product = [&](int m, int i, uint32_t b0, uint32_t b1, const uint32_t (&w)[4]) {
+        if constexpr (f32) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_16<K>(d, w, b0, b1);
+            out[m][i][0] += d[0] + d[2];
+            out[m][i][1] += d[1] + d[3];
+        } else {
+            mma_16<K>(out[m][i], w, b0, b1);
+        }
+    };
     int began = a0, taken = 0;          // the unit with which the warp's part of the item began; items so far
     // tile n is used, then the copy of tile n + kStages requested into its place
 #pragma unroll 1
@@ -227,7 +243,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 #pragma unroll
                 for (int i = 0; i < kOut; i++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) out[m][i][c] = 0.0f;
+                    for (int c = 0; c < kSums; c++) out[m][i][c] = 0.0f;
             }
         }
         if (!mbar_wait_bounded(&bars[warp][stage], (uint32_t)phase, err, 83)) break;
@@ -307,7 +323,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 #pragma unroll
                 for (int i = 0; i < kOut; i++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) out[m][i][c] *= down;
+                    for (int c = 0; c < kSums; c++) out[m][i][c] *= down;
             }
         }
 #pragma unroll
@@ -331,8 +347,8 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int m = 0; m < MT; m++) {
-                        mma_16<K>(out[m][2 * (i0 + i)], w[m], b[i][0], b[i][1]);
-                        mma_16<K>(out[m][2 * (i0 + i) + 1], w[m], b[i][2], b[i][3]);
+                        product(m, 2 * (i0 + i), b[i][0], b[i][1], w[m]);
+                        product(m, 2 * (i0 + i) + 1, b[i][2], b[i][3], w[m]);
                     }
             }
         }
@@ -356,7 +372,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 A* o = static_cast<A*>(p.o) + (size_t)tok * p.ld_o + h * p.dim;
 #pragma unroll
                 for (int i = 0; i < kOut; i++)
-                    if (8 * i + 2 * t4 < p.dim) store_two<A>(o + 8 * i + 2 * t4, (out[m][i][0] + out[m][i][2]) * inv, (out[m][i][1] + out[m][i][3]) * inv);
+                    if (8 * i + 2 * t4 < p.dim) store_two<A>(o + 8 * i + 2 * t4, result(m, i, 0) * inv, result(m, i, 1) * inv);
             } else if (all) {
                 dst = (it.job.prefix ? p.prefix_o : p.own_o) + row * DP;
                 if (t4 == 0) (it.job.prefix ? p.prefix_ml : p.own_ml)[row] = make_float2(top[m], l);
@@ -372,7 +388,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             if (all && t4 == 0) (it.job.prefix ? p.prefix : p.own)[row] = make_int4(cta, 1, 0, it.job.joined && !it.job.prefix ? kJoinPrefix : 0);
             if (dst)
 #pragma unroll
-                for (int i = 0; i < kOut; i++) store_two<float>(dst + 8 * i + 2 * t4, out[m][i][0] + out[m][i][2], out[m][i][1] + out[m][i][3]);
+                for (int i = 0; i < kOut; i++) store_two<float>(dst + 8 * i + 2 * t4, result(m, i, 0), result(m, i, 1));
         }
         }
         __syncwarp();
