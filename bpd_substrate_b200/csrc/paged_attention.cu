@@ -24,14 +24,19 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedArgs p)
     const long rows = (long)p.n_tokens * p.heads, stride = kFew ? (long)gridDim.x : (long)gridDim.x * kJoinGroups;
     pdl_wait();
     pdl_launch_dependents();
+    // (where bounds run backwards, a row may have no job in its group, or several)
+    auto sane = [&](const int4& e) { return e.x >= 0 && e.y >= 0 && e.x <= p.ctas - e.y && e.z >= 0 && e.z < (e.w & kJoinTile ? kTileRows : kSplitRows); };
     long row = kFew ? (long)blockIdx.x : (long)blockIdx.x * kJoinGroups + group;
     int4 next = row < rows ? p.own[row] : make_int4(0, 0, 0, 0);
     for (; row < rows; row += stride) {
         const int4 own = next;
         if (row + stride < rows) next = p.own[row + stride];
-        if (own.y == 0 || (own.y == 1 && !(own.w & kJoinPrefix))) continue;
+        if (own.y == 0 || (own.y == 1 && !(own.w & kJoinPrefix)) || !sane(own)) continue;
         int4 pre = make_int4(0, 0, 0, 0);
-        if (own.w & kJoinPrefix) pre = p.prefix[row];
+        if (own.w & kJoinPrefix) {
+            pre = p.prefix[row];
+            if (!sane(pre)) pre.y = 0;
+        }
         // part i of the row: its own positions' first, then the prefix's
         const int n = own.y + pre.y;
         auto place = [&](int i, const float*& o, const float2*& ml) {
@@ -164,7 +169,8 @@ static int attention_check(const bpdq_paged_kv* kv, int n_tokens, const bpdq_pag
     if (rc || (rc = check_groups(kv, groups))) return rc;
     // a tile of rows holds a token's at least; units of work are counted in 32 bits
     if (kv->heads / kv->kv_heads > 128 || kv->batch + (groups ? groups->n : 0) > kPagedMaxJobs) return latch(BPDQ_ERR_RANGE);
-    return (double)kv->batch * kv->kv_heads * kv->max_pages * kv->page > 8589934592.0 ? latch(BPDQ_ERR_RANGE) : 0;
+    const double capacity = (double)kv->max_pages * kv->page, tiles = 2.0 * n_tokens / (128 / (kv->heads / kv->kv_heads)) + 2.0 * kv->batch;
+    return kv->batch * kv->kv_heads * capacity > 8589934592.0 || tiles * kv->kv_heads * (capacity / 128 + 3) > 2147483647.0 ? latch(BPDQ_ERR_RANGE) : 0;
 }
 
 static PagedArgs arguments(const bpdq_paged_kv& kv, int n_tokens, const bpdq_paged_groups* groups)
@@ -206,8 +212,8 @@ static int paged_attention(const bpdq_paged_kv* kv, const void* q, int ld_q, voi
     if ((((uintptr_t)q | (uintptr_t)o) & 15) || ld_q % unit || ld_o % unit) return latch(BPDQ_ERR_ALIGN);
     if (n_tokens == 0 || kv->batch == 0) return 0;
     PagedArgs p = arguments(*kv, n_tokens, groups);
-    p.q = q; p.o = o; p.ld_q = ld_q; p.ld_o = ld_o; p.scale = scale; p.cap = cap;
     const int ctas = sm_count();
+    p.q = q; p.o = o; p.ld_q = ld_q; p.ld_o = ld_o; p.scale = scale; p.cap = cap; p.ctas = ctas;
     const Kernels run = kernels(p);
     uint8_t* mem = scratch_take(ws, kScratchPaged, carve(p, nullptr, ctas, run.tile), s, &rc);
     if (!mem) return rc;

@@ -21,6 +21,7 @@ struct PagedArgs {
     int split_rows;             // jobs of up to so many rows are k_paged_split's, the others k_paged_tile's
     int both;                   // this launch's requests bring both halves of 128 dimensions
     int f32;                    // activations
+    int ctas;                   // of a grid, at most
     int mark;                   // this launch says which tokens belong to no sequence
     // scratch
     int4* own;                  // [tokens][heads]: what k_paged_join finds of a row's own positions

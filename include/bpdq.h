@@ -626,7 +626,8 @@ typedef struct {
  * at a sequence's positions, the call's new ones too, have to be finite (those behind a token meet weights of 0).  With fp32 activations queries and weights enter the tensor
  * cores as two fp16 numbers each, and sums of more than 512 keys are added as fp32 numbers: results are within 5e-6 of sum_j w_j |v_j|.  groups NULL: none.  A sequence's sums are split over the GPU by a rule on all lengths of the call: its last bits may depend
  * on what else is in the batch.  Up to 128 query heads per key head, 1280 sequences and
- * groups together; batch * kv_heads * max_pages * page up to 2^33.  Scratch: see "scratch memory" above; its size does not depend on lengths. */
+ * groups together; batch * kv_heads * max_pages * page up to 2^33 and,
+ * in whole numbers, (2 n_tokens / (128 / (heads / kv_heads)) + 2 batch) * kv_heads * (max_pages * page / 128 + 3) below 2^31.  Scratch: see "scratch memory" above; its size does not depend on lengths. */
 int bpd_paged_attention_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* o, int ld_o, int n_tokens, float scale, float cap,
                              const bpdq_paged_groups* groups, void* stream);
 size_t bpdq_paged_attention_workspace_bytes(const bpdq_paged_kv* kv, int n_tokens, const bpdq_paged_groups* groups);

@@ -391,6 +391,30 @@ def test_a_key_without_a_number(lib, act, kv, H, G, D, held, new):
         assert ((got - want).abs() <= tolerance(c, want, size, top, 0.0))[~sees].all()
 
 
+@pytest.mark.parametrize("starts", [[0, 10, 5, 8, 12], [0, 10, 5, 12, 11], [3, 1, 12, 0, 12], [0, 12, 0, 12, 0]])
+def test_bounds_that_run_backwards_inside_a_group(lib, starts):
+    """What makes no sense is passed over and reported, and the next call is right."""
+    c = Cache(4, 2, 64, "bf16", "bf16", 16, [100, 96, 130, 100], [3, 3, 3, 3], 9, shared=[(0, 4, 6)])
+    c.fill()
+    desc = c.upload()
+    q = torch.randn(12, 256, generator=c.gen).bfloat16()
+    want, size, top = attention_oracle(c, q, 0.1, 0.0)
+    bounds, pages = i32([0, 4]), i32([6])
+    g = C.byref(capi.PagedGroups(1, bounds.data_ptr(), pages.data_ptr()))
+    d, o = q.cuda(), torch.zeros(12, 256, dtype=torch.bfloat16, device="cuda")
+    right = c.d_start.clone()
+    c.d_start.copy_(i32(starts))
+    torch.cuda.synchronize()
+    assert lib.bpd_paged_attention_cuda(desc, d.data_ptr(), 256, o.data_ptr(), 256, 12, 0.1, 0.0, g, None) == 0
+    torch.cuda.synchronize()
+    assert lib.bpdq_last_status() == -4
+    lib.bpdq_clear_status()
+    c.d_start.copy_(right)
+    torch.cuda.synchronize()
+    done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), 256, o.data_ptr(), 256, 12, 0.1, 0.0, g, None))
+    assert ((o.double().view(12, 4, 64) - want).abs() <= tolerance(c, want, size, top, 0.0)).all()
+
+
 def test_a_sequence_without_a_page_is_zero(lib):
     c = Cache(4, 2, 64, "bf16", "bf16", 16, [20, 20], [1, 1], 3)
     c.fill()

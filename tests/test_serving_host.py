@@ -85,6 +85,15 @@ def test_attention_beyond_its_range(lib, changes):
     lib.bpdq_clear_status()
 
 
+def test_more_products_than_are_counted(lib):
+    """Four million tokens against two million positions: units of work are counted in 32 bits."""
+    kv = paged(max_pages=1 << 17)
+    assert lib.bpdq_paged_attention_workspace_bytes(C.byref(kv), 1 << 17, None) > 0
+    assert attention(lib, kv, n=1 << 22) == -3
+    assert lib.bpdq_paged_attention_workspace_bytes(C.byref(kv), 1 << 22, None) == 0
+    lib.bpdq_clear_status()
+
+
 def test_no_descriptor_and_no_workspace(lib):
     assert append(lib, None) == -1 and attention(lib, None) == -1
     assert lib.bpdq_paged_attention_workspace_bytes(None, 5, None) == 0
