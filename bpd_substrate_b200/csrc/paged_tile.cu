@@ -24,8 +24,9 @@ constexpr int kPtRows = 128, kPtKeys = 128, kPtStep = 64, kPtPiece = 128 * 64 * 
 constexpr int kPtWarps = 8, kPtThreads = 32 * (4 + kPtWarps);          // three groups of four warps, which have registers of their own size
 constexpr float kPtGrowth = 8.0f;
 // The tensor pipe cuts off what does not fit fp32 of each of its sums, always toward zero: 6000 keys in one go are 4e-6 short.  With fp32 activations a stream
-// puts its sums aside every so many steps, added to the last ones as fp32 numbers round, and begins anew.
-constexpr int kPtFold = 8;
+// puts its sums aside every so many steps, added to the last ones as fp32 numbers round, and begins anew.  (Prompts of 1500 after 4000, error against 64 bits, us: every two
+// steps 0.9e-6, 253; four 1.1e-6, 229; eight 1.6e-6, 213.  Elementary operations in fp32: 1.1e-6.)
+constexpr int kPtFold = 4;
 
 template <int DP> struct PtShape {
     static constexpr int halves = DP / 64, depth = DP == 64 ? 4 : 2;        // blocks of keys (and of values) in shared memory
@@ -273,19 +274,26 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 93)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const float down = aside_top == -INFINITY ? 0.0f : ex2(aside_top - top);
-#pragma unroll 1
-                    for (int c = 0; c < DP; c += 16) {
-                        int ov[16];
-                        tmem_ld(to_ + 128 * s + c, ov);
-                        float4 x[4] = {};
-                        if (t > kPtFold)
+                    // (loads run a piece ahead)
+                    float4 x[8] = {}, next[8];
+                    auto last = [&](float4* x, int c) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) x[j] = __ldcg(aside + (c / 4 + j) * kPtRows);
+                        for (int j = 0; j < 8; j++) x[j] = __ldcg(aside + (c / 4 + j) * kPtRows);
+                    };
+                    if (t > kPtFold) last(x, 0);
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        tmem_ld_32(to_ + 128 * s + c, o);
+                        if (t > kPtFold && c + 32 < DP) last(next, c + 32);
                         tmem_loaded();
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            __stcg(aside + (c / 4 + j) * kPtRows, make_float4(fmaf(x[j].x, down, __int_as_float(ov[4 * j])), fmaf(x[j].y, down, __int_as_float(ov[4 * j + 1])),
-                                                                              fmaf(x[j].z, down, __int_as_float(ov[4 * j + 2])), fmaf(x[j].w, down, __int_as_float(ov[4 * j + 3]))));
+                        for (int j = 0; j < 8; j++)
+                            __stcg(aside + (c / 4 + j) * kPtRows,
+                                   make_float4(fmaf(x[j].x, down, o[4 * j]), fmaf(x[j].y, down, o[4 * j + 1]), fmaf(x[j].z, down, o[4 * j + 2]), fmaf(x[j].w, down, o[4 * j + 3])));
+                        if (t > kPtFold)
+#pragma unroll
+                            for (int j = 0; j < 8; j++) x[j] = next[j];
                     }
                     aside_top = top;
                     if (grown) sum *= ex2(top - now);
