@@ -11,7 +11,8 @@ static int check_groups(const bpdq_paged_kv* kv, const bpdq_paged_groups* g)
 }
 
 // Adds up the parts of rows that the kernels ahead have left in scratch memory: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  Eight threads walk through the
-// parts of a row; or, where there are few rows, a CTA has one row and eight threads every sixteenth part.
+// parts of a row; or, where there are few rows, a CTA has one row and eight threads every sixteenth part.  (192000 rows, a fifth of them in two parts: 14 us.  A
+// call of 2048 rows with a prefix: 53 us with a CTA per row, 64 with eight threads; of 2048 without: 49.0 and 48.4.)
 constexpr int kJoinThreads = 128, kJoinGroups = kJoinThreads / 8;
 
 template <typename A, int DP, bool kFew>
@@ -192,11 +193,14 @@ struct Kernels {
 };
 static Kernels kernels(const PagedArgs& p)
 {
-    // k_paged_split's products of 8 rows or of 16: of 16 where sequences bring between 8 and 16 on average (a few tokens each), which the larger tiles would
-    // be mostly empty with.
+    // k_paged_split's products of 8 rows or of 16, or k_paged_tile, for 9 to 16 rows: where query heads on a key head are more than 8, or a few tokens per sequence.
+    // fp32, 16 rows: 16 sequences of 2000 positions 35 us in k_paged_split and 51 in k_paged_tile, 64 of them 83 and 123.  16-bit types, sixteen heads: 1 of 4000 20.5 and
+    // 19.0, 16 of 2000 34.7 and 32.0, 64 103 and 80; four tokens of four heads: 4 of 4000 24.5 and 27.8, 16 of 2000 39.5 and 43.5, 64 107 and 87 (8 key heads of 128).
     const long average = p.seq_start ? ((long)p.n_tokens * p.share + p.batch - 1) / p.batch : p.share;
     Kernels k;
-    k.split_rows = p.share > kSplitRows ? 0 : (p.share > 8 || (average > 8 && average <= kSplitRows) ? kSplitRows : 8);
+    const bool few = p.f32 || (p.share <= 8 && (long)p.batch * p.kv_heads <= 2L * sm_count());
+    k.split_rows = p.share <= 8 ? 8 : 0;
+    if (few && p.share <= kSplitRows && (p.share > 8 || (average > 8 && average <= kSplitRows))) k.split_rows = kSplitRows;
     k.tile = p.seq_start || p.groups || !k.split_rows;
     return k;
 }

@@ -12,6 +12,9 @@
 // O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8 since the last time.  Weights are rounded to the cache's type: half
 // a step (2^-9 of a bf16 weight on average) of each, which the sum over keys averages to below the result's own rounding.  fp32 activations bring queries and weights as two
 // fp16 numbers each: four products where 16 bits take two, and one tile per item.
+// One prompt of 8000 tokens, 32 heads on 8 of 128 in bf16: 553 us, 945 TFLOP/s of a measured 1688; three portions of 2000 after up to 2000: 143 us with the join (14).  Bound by what
+// the streams and the tensor pipe hand to each other: 2500 cycles for a step of both streams, 1024 of them products.  64 tokens on a prefix of 16000 (8 items on 148
+// CTAs): 40 us, half of it until the first scores.
 #include "paged_attention.cuh"
 #include "tcgen05_device.cuh"
 #include "mma_device.cuh"

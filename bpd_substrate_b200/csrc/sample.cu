@@ -7,6 +7,8 @@
 // numbers of 15 bits a weight, as shared memory adds 32): the bins above are settled, the few elements of the bin that holds the cut are listed in one
 // CTA and compared with each other.  Where those are too many (flat rows, equal values) the bin is halved by exact sums until they are not.  Its own
 // histogram tells a CTA what it holds of the kept weights, so only the one with the chosen token walks through them.
+// Bound by the steps that follow one another, each with a meeting of the cluster, and by barriers in them: a row of 32000 11 to 14 us, 64 rows of 128256 57 (their
+// bytes: 5), 300 rows of 32000 in bf16 76, two full waves and a third of four rows.
 #include "cluster_device.cuh"
 #include "launch.cuh"
 #include "paged.cuh"
@@ -470,7 +472,7 @@ __device__ __forceinline__ void cut_in_list(Sampler& w, const Border& b)
             __syncthreads();
             const int parts = Sampler::parts_for(n), j = w.tid / parts;
             ulonglong2 mine = make_ulonglong2(0, 0);
-                if (j < n) mine = s.pair[j];
+            if (j < n) mine = s.pair[j];
             int ahead;
             u64 mass;
             w.counted(n, parts, mine.x, ahead, mass);
