@@ -8,12 +8,14 @@
 //   warps 4-11  softmax, four per stream, a thread per row; weights go back to tensor memory over the scores they came from.  (The tensor pipe works
 //               its products off in the order in which they are issued: scores do not overtake the product that reads the weights beneath them.)
 // (Every barrier of a stream's steps comes twice, for even and odd ones: a role may be two steps ahead of another.)
-// The streams take their exponentials in turns: both at once would wait for the special function unit together and leave it idle together.
+// The streams take their exponentials in turns, the next one from the middle of the other's on: both at once would wait for the special function unit together and leave it
+// idle together.  (One prompt of 8000 tokens: 522 us, one whole step after the other 524, no turns 560; every eighth, fourth or second pair by a polynomial instead of
+// that unit 530, 550, 603: instructions are scarcer.)
 // O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8 since the last time.  Weights are rounded to the cache's type: half
 // a step (2^-9 of a bf16 weight on average) of each, which the sum over keys averages to below the result's own rounding.  fp32 activations bring queries and weights as two
 // fp16 numbers each: four products where 16 bits take two, and one tile per item.
-// One prompt of 8000 tokens, 32 heads on 8 of 128 in bf16: 553 us, 945 TFLOP/s of a measured 1688; three portions of 2000 after up to 2000: 143 us with the join (14).  Bound by what
-// the streams and the tensor pipe hand to each other: 2500 cycles for a step of both streams, 1024 of them products.  64 tokens on a prefix of 16000 (8 items on 148
+// One prompt of 8000 tokens, 32 heads on 8 of 128 in bf16: 522 us, 1005 TFLOP/s of a measured 1688; three portions of 2000 after up to 2000: 133 us with the join (14).  Bound by what
+// the streams and the tensor pipe hand to each other: some 2400 cycles for a step of both streams, 1024 of them products.  64 tokens on a prefix of 16000 (8 items on 148
 // CTAs): 40 us, half of it until the first scores.
 #include "paged_attention.cuh"
 #include "tcgen05_device.cuh"
@@ -79,22 +81,6 @@ __device__ __forceinline__ float2 add_two(float2 a, float2 b)
     return d;
 }
 
-// 2^x of two numbers without the special function unit: x = n + f, |f| <= 1/2, and a polynomial of degree 4 (fitted over that range, off by 3e-6: a weight
-// keeps 8 to 11 bits).  0 from 2^-127 down.
-__device__ __forceinline__ float2 ex2_two(float2 x)
-{
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.0f));        // (a NaN stays one)
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.0f));
-    const float2 shift = make_float2(12582912.0f, 12582912.0f), back = make_float2(-12582912.0f, -12582912.0f), minus = make_float2(-1.0f, -1.0f);
-    const float2 k = add_two(x, shift), f = fma_two(add_two(k, back), minus, x);
-    float2 p = make_float2(9.5605102e-3f, 9.5605102e-3f);
-    p = fma_two(p, f, make_float2(5.5917039e-2f, 5.5917039e-2f));
-    p = fma_two(p, f, make_float2(2.4024981e-1f, 2.4024981e-1f));
-    p = fma_two(p, f, make_float2(6.9312197e-1f, 6.9312197e-1f));
-    p = fma_two(p, f, make_float2(9.9999919e-1f, 9.9999919e-1f));
-    const float2 n = make_float2(__int_as_float((__float_as_int(k.x) << 23) + 0x3F800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3F800000));
-    return fma_two(p, n, make_float2(0.0f, 0.0f));
-}
 // An item: a key head's rows of some tokens of a job.
 struct PtItem {
     PagedJob job;
@@ -106,7 +92,7 @@ struct PtItem {
 constexpr int kPtItems = 4;             // a warp finds the items and puts them here; the others take them
 constexpr int kPtTakers = 1 + 2 + 8;
 // An item's beginning and end (queries, a pipe that runs empty, results) take about as long as two blocks: it counts two units more than it has blocks, its first ones.
-// (One prompt of 8000 tokens, 32 heads on 8 of 128: none 692 us, one 595, two 555, three 555, eight 592.)
+// (One prompt of 8000 tokens, 32 heads on 8 of 128: none 692 us, one 595, two 555, three 555, eight 592, all with a polynomial for every fourth pair of exponentials.)
 constexpr int kPtExtra = 2;
 
 template <typename A, typename K, int DP, bool kCap>
@@ -326,12 +312,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll
                     for (int j = 32 * c; j < 32 * c + 32; j += 2) {
                         float2 x = fma_two(make_float2(v[j], v[j + 1]), f2, zero2);
-                        if (!f32 && (j & 6) == 6) {
-                            x = ex2_two(x);             // every fourth pair, on pipes that the others leave idle
-                        } else {
-                            x.x = ex2(x.x);
-                            x.y = ex2(x.y);
-                        }
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
                         part[(j >> 1) & 1] = add_two(part[(j >> 1) & 1], x);
                         v[j] = x.x;
                         v[j + 1] = x.y;
@@ -347,8 +329,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         for (int j = 0; j < 16; j++) hi[j] = pack_16<K>(v[32 * c + 2 * j], v[32 * c + 2 * j + 1]);
                     }
                     tmem_st(ts + 16 * c, hi);
+                    if (c == 0 && lane == 0) mbar_arrive(&turn[1 - s]);
                 }
-                if (lane == 0) mbar_arrive(&turn[1 - s]);
                 sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
                 if (key + kPtStep > it.job.to || missing) {
                     // whatever lies in places that hold no position must not meet a weight, not even one of 0: two threads per key
