@@ -10,7 +10,7 @@
 // (Every barrier of a stream's steps comes twice, for even and odd ones: a role may be two steps ahead of another.)
 // The streams take their exponentials in turns, the next one from the middle of the other's on: both at once would wait for the special function unit together and leave it
 // idle together.  (One prompt of 8000 tokens: 522 us, one whole step after the other 524, no turns 560; every eighth, fourth or second pair by a polynomial instead of
-// that unit 530, 550, 603: instructions are scarcer.)
+// that unit 530, 550, 603: instructions are scarcer; the scores of a block's 128 keys in one product, into both sets, once both are free 627.)
 // O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8 since the last time.  Weights are rounded to the cache's type: half
 // a step (2^-9 of a bf16 weight on average) of each, which the sum over keys averages to below the result's own rounding.  fp32 activations bring queries and weights as two
 // fp16 numbers each: four products where 16 bits take two, and one tile per item.
