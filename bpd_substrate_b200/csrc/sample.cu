@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
     // ---- the row, and its first place
     const float temperature = p.temperature ? p.temperature[row] : 1.0f;
     const int k = p.top_k ? p.top_k[row] : 0;
-    const float part = p.top_p ? p.top_p[row] : 1.0f, least = p.min_p ? fminf(p.min_p[row], 1.0f) : 0.0f;
+    const float part = p.top_p ? p.top_p[row] : 1.0f, least = p.min_p && p.min_p[row] > 0.0f ? fminf(p.min_p[row], 1.0f) : 0.0f;       // (a setting that is NaN is none)
     const double u = fmin(fmax((double)p.u[row], 0.0), 1.0 - 1.0 / 16777216.0);
     float best = -INFINITY;
     int best_at = 0x7FFFFFFF;

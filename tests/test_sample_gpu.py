@@ -222,3 +222,10 @@ def test_a_row_does_not_depend_on_its_batch_and_graphs_replay(lib):
         assert torch.equal(out, want)
     lib.bpdq_graph_destroy(g)
     lib.bpdq_stream_destroy(s)
+
+
+def test_settings_that_are_no_numbers(lib):
+    """NaN is no cut, and no temperature above 0; shares below 0 are the least ones."""
+    nan = float("nan")
+    x = np.random.default_rng(5).normal(0, 2, (6, 3000)).astype(np.float32)
+    check(lib, x, "f32", t=[1, 1, nan, 0.7, 1, 1], k=[0, 50, 0, 0, 0, 0], p=[nan, nan, 0.9, 0.8, -1, 1], m=[0.01, nan, 0.1, nan, 0, -0.5], u=[0.1, 0.4, 0.6, 0.9, 0.99, 0.7])
