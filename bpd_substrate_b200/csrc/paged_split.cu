@@ -4,6 +4,8 @@
 // do not matter and no warp waits for another before the end.  A warp fills its own ring of tiles (keys and values, tiled bulk copies straight from the
 // pages), and has running maxima, sums and outputs of its rows in registers.  Eight rows fill half of an m16n8k16 product: the other half is the small
 // part of what does not fit 16 bits, of softmax weights (w = hi + lo) and of fp32 queries, so it costs nothing.
+// fp16 ends at 2^16 and rounds what is below 2^-25 to 0.  Weights may reach 2^8 (kPsGrowth), so fp16 ones are held 2^7 times as large, and their small parts, whose
+// products have sums of their own, another 2^11 times: a weight is off by 2^-43 of the largest at most, or by 2^-23 of itself.
 // 64 sequences of up to 8000 positions (8 key heads of 128 in bf16, 796 MB): 136 us with the join, 5.9 TB/s, bound by memory.  One of 4000: 13.8 us, a chain of the plan, the
 // first copies, three tiles a warp and two joins.
 #include "paged_attention.cuh"
@@ -15,6 +17,10 @@ namespace bpdq {
 constexpr int kPsWarps = kSplitWarps, kPsThreads = 32 * kPsWarps, kPsKeys = 16, kPsRing = 24576;        // bytes of a warp's ring
 constexpr int kPsItems = 8;                         // more than copies can be ahead (six tiles)
 constexpr float kPsGrowth = 8.0f;                   // log2 of how far weights may exceed 1 before outputs are rescaled
+template <typename K> constexpr float kPsShift = 0.0f;                  // log2 of what weights are multiplied by on their way to the tensor cores
+template <> constexpr float kPsShift<__half> = 7.0f;
+template <typename K> constexpr float kPsLow = 1.0f;                    // and of their small parts' products: what they are divided by again
+template <> constexpr float kPsLow<__half> = 1.0f / 2048.0f;
 
 template <typename K> __device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma_16<bf16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -36,6 +42,15 @@ template <> __device__ __forceinline__ void split_16<__half>(float v0, float v1,
     const __half2 h = __floats2half2_rn(v0, v1);
     const float2 f = __half22float2(h);
     const __half2 l = __floats2half2_rn(v0 - f.x, v1 - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+template <typename K> __device__ __forceinline__ void split_weights(float v0, float v1, uint32_t& hi, uint32_t& lo) { split_bf16(v0, v1, hi, lo); }
+template <> __device__ __forceinline__ void split_weights<__half>(float v0, float v1, uint32_t& hi, uint32_t& lo)
+{
+    const __half2 h = __floats2half2_rn(v0, v1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn((v0 - f.x) * (1.0f / kPsLow<__half>), (v1 - f.y) * (1.0f / kPsLow<__half>));
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -218,14 +233,14 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     float out[MT][kOut][kSums], top[MT], sum[MT];
     auto result = [&](int m, int i, int c) {
         if constexpr (f32) return out[m][i][c];
-        else return out[m][i][c] + out[m][i][c + 2];
+        else return fmaf(out[m][i][c + 2], kPsLow<K>, out[m][i][c]);
     };
     auto product = [&](int m, int i, uint32_t b0, uint32_t b1, const uint32_t (&w)[4]) {
         if constexpr (f32) {
             float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma_16<K>(d, w, b0, b1);
-            out[m][i][0] += d[0] + d[2];
-            out[m][i][1] += d[1] + d[3];
+            out[m][i][0] += fmaf(d[2], kPsLow<K>, d[0]);
+            out[m][i][1] += fmaf(d[3], kPsLow<K>, d[1]);
         } else {
             mma_16<K>(out[m][i], w, b0, b1);
         }
@@ -332,13 +347,13 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            const float base = top[m] == -INFINITY ? 0.0f : top[m];
+            const float base = top[m] == -INFINITY ? 0.0f : top[m] - kPsShift<K>;
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = ex2(sc[m][i >> 1][i & 1] - base);
             sum[m] += (x[0] + x[1]) + (x[2] + x[3]);
-            split_16<K>(x[0], x[1], w[m][0], w[m][1]);
-            split_16<K>(x[2], x[3], w[m][2], w[m][3]);
+            split_weights<K>(x[0], x[1], w[m][0], w[m][1]);
+            split_weights<K>(x[2], x[3], w[m][2], w[m][3]);
         }
         {
             const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = lane >> 4;
@@ -365,7 +380,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            const float l = quad_sum(sum[m]);
+            const float l = quad_sum(sum[m]), most = top[m] - kPsShift<K>;      // (the maximum that the sums count from)
             const int r = 8 * m + g;
             if (r >= it.job.rows) continue;
             const int tok = it.job.first + row_tok[m], h = it.head * p.share + row_head[m];
@@ -379,15 +394,15 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     if (8 * i + 2 * t4 < p.dim) store_two<A>(o + 8 * i + 2 * t4, result(m, i, 0) * inv, result(m, i, 1) * inv);
             } else if (all) {
                 dst = (it.job.prefix ? p.prefix_o : p.own_o) + row * DP;
-                if (t4 == 0) (it.job.prefix ? p.prefix_ml : p.own_ml)[row] = make_float2(top[m], l);
+                if (t4 == 0) (it.job.prefix ? p.prefix_ml : p.own_ml)[row] = make_float2(most, l);
             } else if (tail) {
                 float* mine = reinterpret_cast<float*>(ring_ptr + warp * kPsRing);
                 dst = mine + r * DP;
-                if (t4 == 0) reinterpret_cast<float2*>(mine + kSplitRows * DP)[r] = make_float2(top[m], l);
+                if (t4 == 0) reinterpret_cast<float2*>(mine + kSplitRows * DP)[r] = make_float2(most, l);
             } else {
                 const size_t at = (size_t)(cta * kPsWarps + warp) * kSplitRows + r;
                 dst = p.head_o + at * DP;
-                if (t4 == 0) p.head_ml[at] = make_float2(top[m], l);
+                if (t4 == 0) p.head_ml[at] = make_float2(most, l);
             }
             if (all && t4 == 0) (it.job.prefix ? p.prefix : p.own)[row] = make_int4(cta, 1, 0, it.job.joined && !it.job.prefix ? kJoinPrefix : 0);
             if (dst)

@@ -11,7 +11,7 @@
 // The streams take their exponentials in turns, the next one from the middle of the other's on: both at once would wait for the special function unit together and leave it
 // idle together.  (One prompt of 8000 tokens: 522 us, one whole step after the other 524, no turns 560; every eighth, fourth or second pair by a polynomial instead of
 // that unit 530, 550, 603: instructions are scarcer; the scores of a block's 128 keys in one product, into both sets, once both are free 627.)
-// O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8 since the last time.  Weights are rounded to the cache's type: half
+// O stays in tensor memory and is rescaled only when a row's maximum has grown by much since the last time.  Weights are rounded to the cache's type: half
 // a step (2^-9 of a bf16 weight on average) of each, which the sum over keys averages to below the result's own rounding.  fp32 activations bring queries and weights as two
 // fp16 numbers each: four products where 16 bits take two, and one tile per item.
 // One prompt of 8000 tokens, 32 heads on 8 of 128 in bf16: 522 us, 1005 TFLOP/s of a measured 1688; three portions of 2000 after up to 2000: 133 us with the join (14).  Bound by what
@@ -27,7 +27,14 @@ namespace bpdq {
 
 constexpr int kPtRows = 128, kPtKeys = 128, kPtStep = 64, kPtPiece = 128 * 64 * 2;     // rows of a tile, keys of a block and of a step, bytes of 128 rows x 64 columns
 constexpr int kPtWarps = 8, kPtThreads = 32 * (4 + kPtWarps);          // three groups of four warps, which have registers of their own size
-constexpr float kPtGrowth = 8.0f;
+// By activations.  O is rescaled when a row's maximum has grown by more than 2^growth since the last time.  fp16 ends at 2^16 and rounds what is below 2^-25 to 0: fp16 weights are
+// held 2^shift times as large, growth + shift < 16, so that each is off by 2^(-25 - shift) of the largest at most, or by its rounding.  (Growth, shift 4, 11 for 8, 7: three fp16 prompts of
+// 2000 after 2000, 32 heads on 8 of 128, 139.1 us for 132.2, of fp32 ones of 1000 156.7 for 155.6; 0, 15: 159.2 and 159.5.)
+template <typename A> constexpr float kPtGrowth = 8.0f;
+template <> constexpr float kPtGrowth<float> = 4.0f;
+template <typename A> constexpr float kPtShift = 0.0f;
+template <> constexpr float kPtShift<__half> = 7.0f;
+template <> constexpr float kPtShift<float> = 11.0f;
 // The tensor pipe cuts off what does not fit fp32 of each of its sums, always toward zero: 6000 keys in one go are 4e-6 short.  With fp32 activations a stream
 // puts its sums aside every so many steps, added to the last ones as fp32 numbers round, and begins anew.  (Prompts of 1500 after 4000, error against 64 bits, us: every two
 // steps 0.9e-6, 253; four 1.1e-6, 229; eight 1.6e-6, 213.  Elementary operations in fp32: 1.1e-6.)
@@ -257,7 +264,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     for (int i = 0; i < 4; i++) m4[i] = j + 4 < 64 ? fmaxf(fmaxf(m4[i], v[j + i]), v[(j + 4 + i) & 63]) : fmaxf(m4[i], v[j + i]);
                 }
                 const float now = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * ff;
-                const bool grown = now > top + kPtGrowth;
+                const bool grown = now > top + kPtGrowth<A>;
                 const bool fold = f32 && t > 0 && t % kPtFold == 0;
                 if (fold) {
                     if (!mbar_wait_bounded(&o_done[s][(steps - 1) & 1], (uint32_t)((steps - 1) >> 1) & 1u, err, 93)) { ok = false; break; }
@@ -303,7 +310,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     }
                 }
                 if (grown) top = now;
-                const float zero = top == -INFINITY ? 0.0f : top;
+                const float zero = top == -INFINITY ? 0.0f : top - kPtShift<A>;
                 if (!mbar_wait_bounded(&turn[s], (uint32_t)steps & 1u, err, 98)) { ok = false; break; }
                 const float2 f2 = make_float2(ff, ff), zero2 = make_float2(-zero, -zero);
                 float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -450,7 +457,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 __syncwarp();
             }
             if (live) {
-                if (!direct) (!all ? p.tile_ml : (it.job.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top, sum);
+                if (!direct) (!all ? p.tile_ml : (it.job.prefix ? p.prefix_ml : p.own_ml))[at] = make_float2(top - kPtShift<A>, sum);
                 if (starts) {
                     const int end = all ? cta : deal.cta_of(it.end - 1);
                     (it.job.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, in_part, kJoinTile | (it.job.joined && !it.job.prefix ? kJoinPrefix : 0));

@@ -623,8 +623,12 @@ typedef struct {
 } bpdq_paged_groups;
 /* o[t][h] = sum_j softmax_j(s_j) v_j over the positions up to the token's own, s = scale q.k, with cap > 0 then cap tanh(s / cap).  The tokens' own keys and values are in the cache
  * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q.  What lies in a page's other places is never looked at; the values
- * at a sequence's positions, the call's new ones too, have to be finite (those behind a token meet weights of 0).  With fp32 activations queries and weights enter the tensor
- * cores as two fp16 numbers each, and sums of more than 256 keys are added as fp32 numbers: results are within 5e-6 of sum_j w_j |v_j|.  groups NULL: none.  A sequence's sums are split over the GPU by a rule on all lengths of the call: its last bits may depend
+ * at a sequence's positions, the call's new ones too, have to be finite (those behind a token meet weights of 0). 
+ * How exact: scores are off by up to (dim + 16) 2^-24 |scale| sum_i |q_i k_i|, and a weight by as much of itself.  With fp32 activations queries and weights enter the tensor cores as two
+ * fp16 numbers each, and sums of more than 256 keys are added as fp32 numbers: beyond what scores are off by, results are within 5e-6 of sum_j w_j |v_j| and, since fp16 has an end, 2^-36 of
+ * w_max sum_j |v_j|.  With 16-bit types weights may be rounded to the cache's type (where a sequence or a group has more than 8 rows): half a step of it of sum_j w_j |v_j|, of fp16
+ * also 2^-32 of w_max sum_j |v_j|, and the result's rounding.
+ * groups NULL: none.  A sequence's sums are split over the GPU by a rule on all lengths of the call: its last bits may depend
  * on what else is in the batch.  Up to 128 query heads per key head, 1280 sequences and
  * groups together; batch * kv_heads * max_pages * page up to 2^33 and,
  * in whole numbers, (2 n_tokens / (128 / (heads / kv_heads)) + 2 batch) * kv_heads * (max_pages * page / 128 + 3) below 2^31.  Scratch: see "scratch memory" above; its size does not depend on lengths. */

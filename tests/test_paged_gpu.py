@@ -662,3 +662,60 @@ def test_a_batch_decodes(lib):
             s.append(x)
         if step == 0:
             assert sequences[2][-1] == int(logits[2].argmax())
+
+
+# ---- rows in which one position takes nearly all
+
+def one_that_takes_nearly_all(c, gap, place, value):
+    """Every sequence's position `place` (the last one, where there are fewer) scores `gap`, all others 0, exactly; it has the value given, the others positive ones."""
+    c.fill()
+    c.v.abs_()
+    for b, (h, n) in enumerate(zip(c.held, c.new)):
+        p = torch.arange(h + n)
+        rows = c.table[b].long()[p // c.page]
+        c.k[rows, :, p % c.page] = 0
+        p = min(place, h)
+        c.k[c.table[b, p // c.page].long(), :, p % c.page, 0] = gap
+        c.v[c.table[b, p // c.page].long(), :, p % c.page] = value
+    q = torch.randn(c.tokens, c.H, c.D, generator=c.gen)
+    q[..., 0] = 1.0
+    return q.reshape(c.tokens, -1).to(TYPES[c.act][0])
+
+
+SMALL = [
+    # (H, G, D, held, new, ranges that share pages): the kernel for few rows with one product and with two, the one for many, both in a call
+    (8, 2, 128, [4000, 16000, 700], [1, 1, 1], ()),
+    (8, 2, 64, [4000, 9000], [4, 4], ()),
+    (4, 2, 128, [3000, 9000], [70, 100], ()),
+    (4, 4, 64, [3000, 9000], [140, 1], ()),
+    (8, 2, 128, [8000] * 9, [1] * 9, [(0, 9, 490)]),
+]
+
+
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("gap", [11.0, 14.0, 17.5, 20.0])
+@pytest.mark.parametrize("place", [0, 2500])
+@pytest.mark.parametrize("value", [0.0, 1.0])
+def test_small_weights(lib, act, kv, gap, place, value):
+    """Weights far below the largest, thousands of them, are not lost.  With fp32 activations: 5e-6 of sum w |v|, 2^-36 of the largest weight on each, three roundings of the
+    score (2^-24 of it each) and of the result.  16-bit types: weights rounded to half a step of the cache's type, of fp16 and 2^-32 of the largest."""
+    for H, G, D, held, new, shared in SMALL:
+        c = Cache(H, G, D, act, kv, 16, held, new, 5, shared=shared)
+        q = one_that_takes_nearly_all(c, gap, place, value)
+        desc, d = c.upload(), q.cuda()
+        o = torch.full_like(d, 9.0)
+        g = None
+        if shared:
+            starts, pages = i32([first for first, _, _ in shared] + [shared[-1][1]]), i32([n for _, _, n in shared])
+            g = C.byref(capi.PagedGroups(len(shared), starts.data_ptr(), pages.data_ptr()))
+        want, size, _ = attention_oracle(c, q, 1.0, 0.0)
+        total = torch.zeros_like(want)
+        for b, (h, n) in enumerate(zip(c.held, c.new)):
+            p = torch.arange(h + n)
+            total[c.start[b]:c.start[b] + n] = c.v[c.table[b].long()[p // 16], :, p % 16].double().sum(0).repeat_interleave(H // G, 0).cuda()
+        done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), H * D, o.data_ptr(), H * D, c.tokens, 1.0, 0.0, g, None))
+        part = {"f32": 5e-6, "f16": 2.0 ** -11 + 2.0 ** -20, "bf16": 2.0 ** -8 + 2.0 ** -20}[act] + 2 * 3 * 2.0 ** -24 * gap
+        floor = {"f32": 2.0 ** -36, "f16": 2.0 ** -32, "bf16": 0.0}[act]
+        bound = HALF_STEP[act] * want + part * size + floor * total + (2.0 ** -25 if act == "f16" else 0)
+        worst = ((o.double().view_as(want) - want).abs() / bound).amax().item()
+        assert worst <= 1, (H, G, D, worst)
