@@ -89,7 +89,7 @@ struct PagedJob {
 struct PagedPlan {
     int* cum;                       // shared, [jobs + 1]
     int* group_len;                 // shared, [groups]: positions that a group shares
-    int4* spans;                    // shared, [jobs]: first token, number of tokens, positions from, to
+    int4* spans;                    // shared, [jobs]: first token, number of tokens, positions from, to; of a group's job, which starts at 0, the sequence whose pages are read instead
     int jobs;
 
     __host__ __device__ static int size(const PagedArgs& p) { return 16 * (p.batch + p.groups) + 4 * (p.batch + 2 * p.groups + 1); }
@@ -132,7 +132,7 @@ struct PagedPlan {
             const int a = p.seq_start ? p.seq_start[s0] : s0, b = p.seq_start ? p.seq_start[s1] : s1;
             r.first = min(max(a, 0), p.n_tokens);
             r.count = min(max(b, r.first), p.n_tokens) - r.first;
-            r.seq = min(s0, p.batch - 1);
+            r.seq = spans[j].z;
             r.from = 0;
             r.to = group_len[j - p.batch];
             r.joined = true;
@@ -145,7 +145,7 @@ struct PagedPlan {
     {
         if (p.mark && blockIdx.x == 0 && !p.seq_start && !r.prefix && r.count == 0)
             for (int h = 0; h < p.heads; h++) p.own[(size_t)j * p.heads + h] = make_int4(0, 0, 0, 0);
-        spans[j] = make_int4(r.first, r.count, r.from, r.to);
+        spans[j] = make_int4(r.first, r.count, r.prefix ? r.seq : r.from, r.to);
     }
     // Job j, once the plan is built.
     __device__ __forceinline__ PagedJob known(const PagedArgs& p, int j) const
@@ -153,15 +153,10 @@ struct PagedPlan {
         const int4 s = spans[j];
         PagedJob r;
         r.prefix = j >= p.batch;
-        r.first = s.x; r.count = s.y; r.from = s.z; r.to = s.w;
+        r.first = s.x; r.count = s.y; r.from = r.prefix ? 0 : s.z; r.to = s.w;
         r.rows = r.count * p.share;
         r.joined = r.prefix || r.from > 0;
-        r.seq = j;
-        if (r.prefix) {
-            int s0, s1;
-            members(p, j - p.batch, s0, s1);
-            r.seq = min(s0, p.batch - 1);
-        }
+        r.seq = r.prefix ? s.z : j;
         return r;
     }
     // units(job): those of one of its items, 0 for a job that is not this kernel's.  All threads of the CTA; returns the units in all.
@@ -175,19 +170,26 @@ struct PagedPlan {
         cum = shared + 4 * jobs;
         group_len = cum + jobs + 1;
         if (p.groups) {
-            for (int g = tid; g < p.groups; g += kThreads) group_len[g] = min(max(p.group_pages[g], 0), p.max_pages) * p.page;
+            // What a group shares is its members' that bring tokens: their least length, the first one's pages.  (Another's row of the table may name anything.)
+            for (int g = tid; g < p.groups; g += kThreads) {
+                group_len[g] = min(max(p.group_pages[g], 0), p.max_pages) * p.page;
+                spans[p.batch + g].z = p.batch;
+            }
             __syncthreads();
             for (int b = tid; b < p.batch; b += kThreads) {
                 const int g = group_of(p, b);
                 if (g < 0) continue;
                 const PagedSpan s = span(p, b, err);
-                if (s.count > 0) atomicMin(&group_len[g], s.held);
+                if (s.count > 0) {
+                    atomicMin(&group_len[g], s.held);
+                    atomicMin(&spans[p.batch + g].z, b);
+                }
             }
             __syncthreads();
             for (int g = tid; g < p.groups; g += kThreads) {
                 int s0, s1;
                 members(p, g, s0, s1);
-                group_len[g] = s1 - s0 > 1 ? group_len[g] / p.page * p.page : 0;
+                group_len[g] = s1 - s0 > 1 && spans[p.batch + g].z < p.batch ? group_len[g] / p.page * p.page : 0;
             }
             __syncthreads();
         }

@@ -615,7 +615,8 @@ typedef struct {
 int bpd_paged_append_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* q_out, int ld_q_out, const void* k, int ld_k, const void* v, int ld_v,
                           int n_tokens, int rot_dims, int neighbours, const float* rot_freq, void* stream);
 /* Sequences that begin with the same pages: sequences start[g] .. start[g + 1] - 1 (start[n] <= batch, n <= batch) share the first pages[g] entries of their rows of
- * page_table, all filled before the call (pages[g] * page <= length of each of them; what goes beyond that is not taken to be shared).  Those keys are then read once for all of the group's
+ * page_table, all filled before the call (pages[g] * page <= length of each of them; what goes beyond that is not taken to be shared).  Only sequences that bring tokens
+ * count: lengths and rows of page_table of others are not looked at.  Those keys are then read once for all of the group's
  * tokens; without it the result is the same up to the order of the sums. */
 typedef struct {
     int n;

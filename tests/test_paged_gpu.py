@@ -719,3 +719,25 @@ def test_small_weights(lib, act, kv, gap, place, value):
         bound = HALF_STEP[act] * want + part * size + floor * total + (2.0 ** -25 if act == "f16" else 0)
         worst = ((o.double().view_as(want) - want).abs() / bound).amax().item()
         assert worst <= 1, (H, G, D, worst)
+
+
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("row", ["cleared", "another's", "short"])
+@pytest.mark.parametrize("new", [[0, 1, 1, 1], [0, 30, 1, 200], [0, 0, 1, 1], [0, 0, 0, 5]])
+def test_groups_whose_first_sequence_brings_nothing(lib, act, kv, row, new):
+    """A slot whose sequence is finished: its row of the table is not what the others share."""
+    held = [0, 640, 700, 655]
+    for H, G, D in ((8, 2, 128), (4, 4, 64)):
+        c = Cache(H, G, D, act, kv, 16, held, new, 7, ragged=True, shared=[(1, 4, 40)])
+        if row != "cleared":
+            c.table[0] = torch.randint(0, c.n_pages, (c.max_pages,), generator=c.gen, dtype=torch.int32)
+        c.held[0] = 5 if row == "short" else 0
+        c.fill()
+        q = torch.randn(c.tokens, H * D, generator=c.gen).to(TYPES[act][0])
+        want, size, top = attention_oracle(c, q, 0.1, 0.0)
+        bounds, pages = i32([0, 4]), i32([40])
+        g = C.byref(capi.PagedGroups(1, bounds.data_ptr(), pages.data_ptr()))
+        desc, d = c.upload(), q.cuda()
+        o = torch.full_like(d, 9.0)
+        done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), H * D, o.data_ptr(), H * D, c.tokens, 0.1, 0.0, g, None))
+        assert ((o.double().view_as(want) - want).abs() <= tolerance(c, want, size, top, 0.0)).all()
