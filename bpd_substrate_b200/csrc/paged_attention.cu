@@ -196,7 +196,7 @@ static Kernels kernels(const PagedArgs& p)
     // k_paged_split's products of 8 rows or of 16, or k_paged_tile, for 9 to 16 rows: where query heads on a key head are more than 8, or a few tokens per sequence.
     // fp32, 16 rows: 16 sequences of 2000 positions 35 us in k_paged_split and 51 in k_paged_tile, 64 of them 83 and 123.  16-bit types, sixteen heads: 1 of 4000 20.5 and
     // 19.0, 16 of 2000 34.7 and 32.0, 64 103 and 80; four tokens of four heads: 4 of 4000 24.5 and 27.8, 16 of 2000 39.5 and 43.5, 64 107 and 87 (8 key heads of 128).
-    const long average = p.seq_start ? ((long)p.n_tokens * p.share + p.batch - 1) / p.batch : p.share;
+    const long average = p.seq_start && p.batch ? ((long)p.n_tokens * p.share + p.batch - 1) / p.batch : p.share;
     Kernels k;
     const bool few = p.f32 || (p.share <= 8 && (long)p.batch * p.kv_heads <= 2L * sm_count());
     k.split_rows = p.share <= 8 ? 8 : 0;

@@ -115,3 +115,16 @@ def test_bad_samples(lib, changes, status):
     a.update(changes)
     assert lib.bpd_sample_cuda(a["logits"], a["type"], a["ld"], a["rows"], a["vocab"], None, None, None, None, a["u"], a["token"], None, None) == status
     lib.bpdq_clear_status()
+
+
+@pytest.mark.parametrize("batch,n,seq_start", [(0, 0, P), (0, 5, P), (3, 0, P), (0, 0, None), (0, 5, None)])
+@pytest.mark.parametrize("types", [(capi.TYPE_BF16, capi.TYPE_BF16), (capi.TYPE_F32, capi.TYPE_F16)])
+def test_scratch_of_an_empty_step(lib, batch, n, seq_start, types):
+    """Its size can be asked for, and a workspace of that size (or any other) does."""
+    kv = paged(batch=batch, seq_start=seq_start, act_type=types[0], kv_type=types[1])
+    size = lib.bpdq_paged_attention_workspace_bytes(C.byref(kv), n, None)
+    assert size > 0
+    g = capi.PagedGroups(0, None, None)
+    assert lib.bpdq_paged_attention_workspace_bytes(C.byref(kv), n, C.byref(g)) == size
+    for given in (size, 16):
+        assert lib.bpd_paged_attention_ws_cuda(C.byref(kv), P, 512, P, 512, n, 0.1, 0.0, None, P, given, None) == 0
