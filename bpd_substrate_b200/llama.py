@@ -219,7 +219,9 @@ class DeviceLlama:
                                                         d_k, d_v, d_logits, d_out, self.stream),
                        "bpd_llama_forward_tiles_cuda")
             if pick is not None:
-                return pick(d_logits)
+                picked = pick(d_logits)             # (which waits for the stream)
+                capi.check(lib.bpdq_last_status(), "llama forward")
+                return picked
             capi.check(lib.bpdq_stream_sync(self.stream))
             logits = np.empty((n, self.cfg.vocab_size), np.float32)
             tokens = np.empty(n, np.int64)

@@ -5,9 +5,10 @@ import json
 import numpy as np
 import pytest
 
-from bpd_substrate_b200 import _build, generate, llama
+from bpd_substrate_b200 import _build, capi, generate, llama
 from bpd_substrate_b200.engine import Engine, Request
 from bpd_substrate_b200.sampling import Sampling
+from bpd_substrate_b200.sequences import Sequence
 from tests import hybrid_models as hm
 from tests import test_hybrid_gpu as hybrid
 from tests.test_hybrid_host import FakeModel
@@ -121,3 +122,45 @@ def test_command(lib, tmp_path, capsys):
     assert said[1] == e.generate([[5, 17, 3], [8]], 6, sampling=Sampling(0.9, 20, 0.9, 0.01, 7))
     e.close()
     m.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sampling", [None, Sampling(0.8, seed=1)])
+def test_a_token_without_an_embedding_raises(lib, sampling):
+    """What the device reports of a step is an error of that step, however its token is chosen."""
+    cfg = llama.make_config(n_layers=1, n_heads=4, n_kv_heads=2, head_dim=32, ffn_dim=256, vocab_size=96, max_seq_len=48)
+    m = llama.DeviceLlama(llama.SyntheticLlama(cfg, seed=3), lib)
+    e = Engine(m, slots=1, portion=8)
+    try:
+        with pytest.raises(capi.BpdqError):
+            e.generate([[5, 96, 7]], 2, sampling=sampling)
+    finally:
+        lib.bpdq_clear_status()
+        e.close()
+        m.close()
+
+
+def test_what_the_device_reports_of_a_sampled_step_is_raised():
+    """The same without a device: the library says after the step that something in it went wrong."""
+    class Lib:
+        status = 0
+
+        def __getattr__(self, name):
+            return lambda *args: 1 << 20 if name == "bpdq_alloc" else 0
+
+        def bpdq_last_status(self):
+            return self.status
+
+    class Sampler:
+        def pick(self, logits, vocab, rule, u):
+            return 7
+
+    m = llama.DeviceLlama.__new__(llama.DeviceLlama)
+    m.lib, m.cfg, m.stream, m.vocab, m.weights, m._sampler = Lib(), llama.make_config(1, 4, 2, 32, 256, 96, 48), None, 96, capi.LlamaWeights(), Sampler()
+    m._offsets = {"k": 0, "v": 0}
+    seq = Sequence(0, 1 << 20, 48)
+    assert m.sample(seq, [1, 2], Sampling(), 0.5) == 7 and seq.length == 2
+    m.lib.status = -4
+    with pytest.raises(capi.BpdqError):
+        m.sample(seq, [3], Sampling(), 0.5)
+    assert seq.length == 2
