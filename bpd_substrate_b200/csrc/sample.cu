@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) k_sample(const SampleArgs p
     float best = -INFINITY;
     int best_at = 0x7FFFFFFF;
     auto take = [&](int i, float v) {
-        if (!(v > -INFINITY)) v = -INFINITY;                     // NaN too
+        v = v > -INFINITY ? v + 0.0f : -INFINITY;                // NaN too; -0 becomes 0, which it is equal to, so that equal numbers have one place by value
         if (v > best) { best = v; best_at = i; }                 // (a thread's indices rise)
         return v;
     };

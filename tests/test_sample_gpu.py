@@ -229,3 +229,19 @@ def test_settings_that_are_no_numbers(lib):
     nan = float("nan")
     x = np.random.default_rng(5).normal(0, 2, (6, 3000)).astype(np.float32)
     check(lib, x, "f32", t=[1, 1, nan, 0.7, 1, 1], k=[0, 50, 0, 0, 0, 0], p=[nan, nan, 0.9, 0.8, -1, 1], m=[0.01, nan, 0.1, nan, 0, -0.5], u=[0.1, 0.4, 0.6, 0.9, 0.99, 0.7])
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("s", SETTINGS, ids=str)
+@pytest.mark.parametrize("t", [0.0, 0.8])
+def test_zeros_of_both_signs(lib, kind, s, t):
+    """They are equal: the lowest index goes first, among the largest logits and at a cut with more of them than are sorted."""
+    rng = np.random.default_rng(18)
+    x = -np.abs(normal(6, 9000, 19)) - 0.5
+    x[0, 5], x[0, 100], x[0, 8000] = -0.0, 0.0, 0.0
+    x[1, [4, 7]], x[1, 2000] = 0.0, -0.0
+    x[2:] = np.where(rng.random((4, 9000)) < 0.5, rng.choice(np.array([0.0, -0.0], np.float32), (4, 9000)), x[2:])
+    x[3:5, ::1000] = 1.0
+    x[5, :4000] = -0.0
+    x[5, 4000:] = 0.0
+    check(lib, x, kind, t=[t] * 6, u=[0.1, 0.5, 0.2, 0.6, 0.9, 0.7], **settings(6, s))
