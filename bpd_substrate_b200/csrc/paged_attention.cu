@@ -229,7 +229,6 @@ static int paged_attention(const bpdq_paged_kv* kv, const void* q, int ld_q, voi
     }
     if (run.split_rows) {
         p.mark = 1;
-        p.behind = run.tile;
         if ((rc = paged_split(p, *kv, ctas, s))) return rc;
     }
     const bool wide = kv->dim > 64;

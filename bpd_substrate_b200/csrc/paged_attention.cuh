@@ -22,7 +22,6 @@ struct PagedArgs {
     int both;                   // this launch's requests bring both halves of 128 dimensions
     int f32;                    // activations
     int ctas;                   // of a grid, at most
-    int behind;                 // k_paged_split: k_paged_tile is the launch before
     int mark;                   // this launch says which tokens belong to no sequence
     // scratch
     int4* own;                  // [tokens][heads]: what k_paged_join finds of a row's own positions

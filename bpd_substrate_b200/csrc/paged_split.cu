@@ -116,9 +116,8 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         row_tok[m] = (8 * m + g) / p.share;
         row_head[m] = 8 * m + g - row_tok[m] * p.share;
     }
-    // Behind k_paged_tile this grid begins on the SMs which that one leaves: it starts when all CTAs of that one have waited for the launches before, so the call's inputs are
-    // there, and neither reads what the other writes.  It does not end before the other has, which is what k_paged_join waits for.
-    if (!p.behind) pdl_wait();
+    // (Behind k_paged_tile too: only a wait makes visible to this grid what launches before that one have written.)
+    pdl_wait();
     pdl_launch_dependents();
 
     PagedPlan plan = {};
@@ -493,7 +492,6 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             (item.prefix ? p.prefix : p.own)[row] = make_int4(cta, end - cta + 1, r, item.joined && !item.prefix ? kJoinPrefix : 0);
         }
     }
-    if (p.behind) pdl_wait();
 }
 
 template <typename A, typename K, int DP, int MT>

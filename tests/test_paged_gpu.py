@@ -741,3 +741,44 @@ def test_groups_whose_first_sequence_brings_nothing(lib, act, kv, row, new):
         o = torch.full_like(d, 9.0)
         done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), H * D, o.data_ptr(), H * D, c.tokens, 0.1, 0.0, g, None))
         assert ((o.double().view_as(want) - want).abs() <= tolerance(c, want, size, top, 0.0)).all()
+
+
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_what_the_launches_before_have_written(lib, act, kv):
+    """A step right behind what fills its cache, queries, lengths and table, prompts and single tokens in one call, again and again without a wait between: the bits
+    that the same steps give one at a time."""
+    H, G, D, new = 8, 2, 128, [1, 90, 1, 1, 200, 1]
+    c = Cache(H, G, D, act, kv, 16, [700, 40, 3000, 95, 0, 16], new, 3, spare_entries=4)
+    c.fill(everything=False)
+    desc, T, ld = c.upload(), c.tokens, (H + 2 * G) * D
+    rows = [torch.randn(T, ld, generator=c.gen).to(TYPES[act][0]).cuda() for _ in range(12)]
+    lengths = [i32([max(0, h - 3 * i) for h in c.held]) for i in range(12)]
+    tables = [c.d_table.clone() for _ in range(12)]
+    for i, t in enumerate(tables):
+        t[:, :1] = t[:, :1].roll(i, 0)
+    x, out = torch.empty_like(rows[0]), [torch.empty(T, H * D, dtype=rows[0].dtype, device="cuda") for _ in range(24)]
+    size, start = x.element_size(), c.d_pool.clone()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def steps(at, wait):
+        with torch.cuda.stream(stream):
+            c.d_pool.copy_(start)
+            for i in range(12):
+                x.copy_(rows[i])
+                c.d_len.copy_(lengths[i])
+                c.d_table.copy_(tables[i])
+                p, s = x.data_ptr(), stream.cuda_stream
+                assert lib.bpd_paged_append_cuda(desc, p, ld, p, ld, p + H * D * size, ld, p + (H + G) * D * size, ld, T, 0, 0, None, s) == 0
+                if wait:
+                    stream.synchronize()
+                assert lib.bpd_paged_attention_cuda(desc, p, ld, out[at + i].data_ptr(), H * D, T, 0.1, 0.0, None, s) == 0
+                if wait:
+                    stream.synchronize()
+        stream.synchronize()
+
+    steps(0, True)
+    for _ in range(5):
+        steps(12, False)
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(out[:12], out[12:]))
+    assert lib.bpdq_last_status() == 0
