@@ -217,7 +217,7 @@ static int paged_attention(const bpdq_paged_kv* kv, const void* q, int ld_q, voi
     if (n_tokens == 0 || kv->batch == 0) return 0;
     PagedArgs p = arguments(*kv, n_tokens, groups);
     const int ctas = sm_count();
-    p.q = q; p.o = o; p.ld_q = ld_q; p.ld_o = ld_o; p.scale = scale; p.cap = cap; p.ctas = ctas;
+    p.q = q; p.o = o; p.ld_q = ld_q; p.ld_o = ld_o; p.scale = scale; p.cap = cap; p.ctas = ctas; p.cap_kind = cap_kind(cap, p.f32);
     const Kernels run = kernels(p);
     uint8_t* mem = scratch_take(ws, kScratchPaged, carve(p, nullptr, ctas, run.tile), s, &rc);
     if (!mem) return rc;

@@ -316,7 +316,8 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 x[i] = sc[m][i >> 1][i & 1] + sc2[m][i >> 1][i & 1];
                 if constexpr (f32) x[i] += sc[m][i >> 1][2 + (i & 1)] + sc2[m][i >> 1][2 + (i & 1)];
                 x[i] *= factor[m];
-                if (p.cap > 0.0f) x[i] = capped<f32>(x[i], p.cap);
+                if (p.cap_kind == kCapNear) x[i] = capped<f32, kCapNear>(x[i], p.cap);
+                else if (p.cap_kind == kCapFar) x[i] = capped<f32, kCapFar>(x[i], p.cap);
                 x[i] *= 1.44269504088896341f;
             }
             if (!whole || it.key + kPsKeys > limit[m]) {

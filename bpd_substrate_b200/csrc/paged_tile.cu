@@ -102,7 +102,7 @@ constexpr int kPtTakers = 1 + 2 + 8;
 // (One prompt of 8000 tokens, 32 heads on 8 of 128: none 692 us, one 595, two 555, three 555, eight 592, all with a polynomial for every fourth pair of exponentials.)
 constexpr int kPtExtra = 2;
 
-template <typename A, typename K, int DP, bool kCap>
+template <typename A, typename K, int DP, int kCap>
 __global__ void __launch_bounds__(kPtThreads, 1)
 k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedArgs p, int* err)
 {
@@ -249,7 +249,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 if (kCap) {
                     const float in = f * 0.69314718055994531f;
 #pragma unroll
-                    for (int j = 0; j < 64; j++) v[j] = capped<f32>(v[j] * in, p.cap) * 1.44269504088896341f;
+                    for (int j = 0; j < 64; j++) v[j] = capped<f32, kCap>(v[j] * in, p.cap) * 1.44269504088896341f;
                     ff = 1.0f;
                 }
                 if (edge) {
@@ -661,7 +661,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     }
 }
 
-template <typename A, typename K, int DP, bool kCap>
+template <typename A, typename K, int DP, int kCap>
 static int launch_tile(PagedArgs a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
 {
     CUtensorMap qmap, kmap, vmap;
@@ -681,8 +681,11 @@ static int launch_tile(PagedArgs a, const bpdq_paged_kv& kv, int ctas, cudaStrea
 template <typename A, typename K>
 static int launch_kind(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)
 {
-    if (a.dim > 64) return a.cap > 0.0f ? launch_tile<A, K, 128, true>(a, kv, ctas, s) : launch_tile<A, K, 128, false>(a, kv, ctas, s);
-    return a.cap > 0.0f ? launch_tile<A, K, 64, true>(a, kv, ctas, s) : launch_tile<A, K, 64, false>(a, kv, ctas, s);
+    const bool wide = a.dim > 64;
+    if (a.cap_kind == kCapNone) return wide ? launch_tile<A, K, 128, kCapNone>(a, kv, ctas, s) : launch_tile<A, K, 64, kCapNone>(a, kv, ctas, s);
+    if constexpr (sizeof(A) == 2)
+        if (a.cap_kind == kCapFar) return wide ? launch_tile<A, K, 128, kCapFar>(a, kv, ctas, s) : launch_tile<A, K, 64, kCapFar>(a, kv, ctas, s);
+    return wide ? launch_tile<A, K, 128, kCapNear>(a, kv, ctas, s) : launch_tile<A, K, 64, kCapNear>(a, kv, ctas, s);
 }
 
 int paged_tile(const PagedArgs& a, const bpdq_paged_kv& kv, int ctas, cudaStream_t s)

@@ -782,3 +782,20 @@ def test_what_the_launches_before_have_written(lib, act, kv):
         steps(12, False)
         assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(out[:12], out[12:]))
     assert lib.bpdq_last_status() == 0
+
+
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("cap", [1e-42, 1e-30, 1e-6, 100.0, 1e5, 1e8, 3e38])
+def test_caps_far_from_the_scores(lib, act, kv, cap):
+    """A cap far above the scores changes nothing, one far below makes all positions alike.  What scores are off by (dim + 8 roundings of sum |q k|, 2^-21 of it by the split of fp32
+    queries) and 2^-20 of what the cap leaves of them."""
+    for new in ([1, 1, 1], [60, 1, 150]):
+        c = Cache(8, 2, 64, act, kv, 16, [3, 500, 60], new, 11)
+        c.fill()
+        q = torch.randn(c.tokens, 512, generator=c.gen).to(TYPES[act][0])
+        want, size, top = attention_oracle(c, q, 0.5, cap)
+        desc, d = c.upload(), q.cuda()
+        o = torch.full_like(d, 9.0)
+        done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), 512, o.data_ptr(), 512, c.tokens, 0.5, cap, None, None))
+        miss = (o.double().view_as(want) - want).abs() - tolerance(c, want, size, top * (1 + 2.0 ** -20 / (c.D * 2.0 ** -24)), 0.0)
+        assert miss.max() <= 0, (new, miss.max().item())
