@@ -176,6 +176,7 @@ extern "C" int bpd_paged_append_cuda(const bpdq_paged_kv* kv, const void* q, int
     const bool f32 = kv->act_type == BPDQ_TYPE_F32;
     const uintptr_t places = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v;
     if (places & (f32 ? 3 : 1)) return latch(BPDQ_ERR_ALIGN);
+    if (q && q == q_out && ld_q != ld_q_out && n_tokens > 1) return latch(BPDQ_ERR_ARG);       // (rows would lie over others that are yet to be read)
     // Four pairs per thread where rows and halves allow loads of four elements (8 bytes, or 16 of fp32).
     const int unit = f32 ? 15 : 7;
     const bool wide = !(places & unit) && !((ld_k | ld_v | (q ? ld_q | ld_q_out : 0)) & 3) && rot_dims % 8 == 0;

@@ -214,6 +214,7 @@ static int paged_attention(const bpdq_paged_kv* kv, const void* q, int ld_q, voi
     if (!q || !o || ld_q < width || ld_o < width || !(cap >= 0.0f) || !isfinite(cap) || !isfinite(scale)) return latch(BPDQ_ERR_ARG);
     const int unit = kv->act_type == BPDQ_TYPE_F32 ? 4 : 8;
     if ((((uintptr_t)q | (uintptr_t)o) & 15) || ld_q % unit || ld_o % unit) return latch(BPDQ_ERR_ALIGN);
+    if (q == o && ld_q != ld_o && n_tokens > 1) return latch(BPDQ_ERR_ARG);         // (rows would lie over others that are yet to be read)
     if (n_tokens == 0 || kv->batch == 0) return 0;
     PagedArgs p = arguments(*kv, n_tokens, groups);
     const int ctas = sm_count();

@@ -609,7 +609,7 @@ typedef struct {
     const int32_t *page_table, *length, *seq_start;
 } bpdq_paged_kv;
 /* The queries q, keys k and values v of n_tokens tokens (rows ld_* elements apart, heads side by side): queries and keys are turned by their
- * positions, queries stored in q_out (which may be q; both NULL: no queries), keys and values in their pages.  Of a head's first rot_dims (even, up
+ * positions, queries stored in q_out (which may be q, with the same ld; both NULL: no queries), keys and values in their pages.  Of a head's first rot_dims (even, up
  * to dim; 0: none) dimensions pair i, dimensions (2 i, 2 i + 1) with neighbours and (i, i + rot_dims / 2) without, turns by position * rot_freq[i]:
  * the Llama's pairing and the hybrid decoders'.  Two tokens must not have the same place. */
 int bpd_paged_append_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* q_out, int ld_q_out, const void* k, int ld_k, const void* v, int ld_v,
@@ -623,7 +623,7 @@ typedef struct {
     const int32_t *start, *pages;
 } bpdq_paged_groups;
 /* o[t][h] = sum_j softmax_j(s_j) v_j over the positions up to the token's own, s = scale q.k, with cap > 0 then cap tanh(s / cap).  The tokens' own keys and values are in the cache
- * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q.  What lies in a page's other places is never looked at; the values
+ * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q, with the same ld.  What lies in a page's other places is never looked at; the values
  * at a sequence's positions, the call's new ones too, have to be finite (those behind a token meet weights of 0). 
  * How exact: scores are off by up to (dim + 16) 2^-24 |scale| sum_i |q_i k_i|, and a weight by as much of itself.  With fp32 activations queries and weights enter the tensor cores as two
  * fp16 numbers each, and sums of more than 256 keys are added as fp32 numbers: beyond what scores are off by, results are within 5e-6 of sum_j w_j |v_j| and, since fp16 has an end, 2^-36 of

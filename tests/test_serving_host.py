@@ -128,3 +128,12 @@ def test_scratch_of_an_empty_step(lib, batch, n, seq_start, types):
     assert lib.bpdq_paged_attention_workspace_bytes(C.byref(kv), n, C.byref(g)) == size
     for given in (size, 16):
         assert lib.bpd_paged_attention_ws_cuda(C.byref(kv), P, 512, P, 512, n, 0.1, 0.0, None, P, given, None) == 0
+
+
+def test_in_place_only_row_by_row(lib):
+    """Results in the place of the queries with other distances between rows would overwrite queries that are still to be read."""
+    kv = paged()
+    assert append(lib, kv, ld_q=512, ld_q_out=640) == -1 and append(lib, kv, ld_q=640, ld_q_out=512) == -1
+    assert attention(lib, kv, ld_q=512, ld_o=640) == -1 and attention(lib, kv, ld_q=640, ld_o=512) == -1
+    assert lib.bpd_paged_attention_ws_cuda(C.byref(kv), P, 512, P, 640, 5, 0.1, 0.0, None, P, 1 << 30, None) == -1
+    lib.bpdq_clear_status()
