@@ -91,7 +91,7 @@ class Engine:
         return picked
 
     def run(self, requests):
-        """Generation of all requests, oldest first into free slots; fills their `output`."""
+        """Generation of all requests, oldest first into free slots; fills their `output`.  Where one fails, its error ends them all and their slots are free again."""
         for i, r in enumerate(requests):
             r.key = ("request", i)
             if not len(r.prompt) or r.max_new_tokens < 1:
@@ -99,15 +99,20 @@ class Engine:
             if len(r.prompt) + r.max_new_tokens - 1 > self.model.capacity:
                 raise ValueError(f"{len(r.prompt)} + {r.max_new_tokens} tokens do not fit a sequence of {self.model.capacity}")
         waiting, running = deque(requests), deque()
-        while waiting or running:
-            while waiting and self.slots.free:
-                running.append(waiting.popleft())
-                self._start(running[-1])
-            r = running.popleft()
-            if self._advance(r):
-                self.end(r.key)
-            else:
-                running.append(r)
+        try:
+            while waiting or running:
+                while waiting and self.slots.free:
+                    running.append(waiting.popleft())
+                    self._start(running[-1])
+                r = running.popleft()
+                if self._advance(r):
+                    self.end(r.key)
+                else:
+                    running.append(r)
+        finally:
+            for r in requests:
+                if r.key in self.live:
+                    self.end(r.key)
         return requests
 
     def _start(self, r):

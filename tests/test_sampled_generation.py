@@ -164,3 +164,18 @@ def test_what_the_device_reports_of_a_sampled_step_is_raised():
     with pytest.raises(capi.BpdqError):
         m.sample(seq, [3], Sampling(), 0.5)
     assert seq.length == 2
+
+
+def test_an_engine_goes_on_after_a_request_that_fails():
+    """Its slot and those of the requests beside it are free again."""
+    e = Engine(SamplingModel(), 2, 4)
+    for _ in range(3):
+        with pytest.raises(ValueError):
+            e.run([Request([1], 5), Request([2, 3], 2, sampling=Sampling(top_k=1)), Request([4], 2)])
+        assert not e.live and len(e.slots.free) == 2
+    assert e.generate([[1], [2], [3]], 3) == [[1, 2, 4], [2, 4, 8], [3, 6, 12]]
+    # a sequence that the caller feeds by itself stays
+    e.feed("mine", [5])
+    with pytest.raises(ValueError):
+        e.generate([[1]], 2, sampling=Sampling(top_k=1))
+    assert list(e.live) == ["mine"] and e.feed("mine", [6], [0])[1].tolist() == [11]
