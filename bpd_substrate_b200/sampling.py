@@ -1,6 +1,7 @@
 """The choice of a token from a row of logits that lies on the device, by temperature, top-k, top-p and min-p (``bpd_sample_cuda``)."""
 import ctypes as C
 from dataclasses import dataclass
+from numbers import Integral
 
 import numpy as np
 
@@ -25,6 +26,8 @@ class Sampling:
             raise ValueError(f"top_p of {self.top_p}: a share of (0, 1]")
         if not 0 <= self.min_p <= 1:
             raise ValueError(f"min_p of {self.min_p}: a share of [0, 1]")
+        if not isinstance(self.seed, Integral) or self.seed < 0:
+            raise ValueError(f"a seed of {self.seed}: a whole number from 0 on")
 
     def numbers(self):
         """A generator of the request's random numbers, `random(dtype=np.float32)` for each token."""

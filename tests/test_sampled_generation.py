@@ -179,3 +179,9 @@ def test_an_engine_goes_on_after_a_request_that_fails():
     with pytest.raises(ValueError):
         e.generate([[1]], 2, sampling=Sampling(top_k=1))
     assert list(e.live) == ["mine"] and e.feed("mine", [6], [0])[1].tolist() == [11]
+
+
+@pytest.mark.parametrize("seed", [-1, 0.5, "one", None])
+def test_seeds_that_make_no_sense(seed):
+    with pytest.raises(ValueError):
+        Sampling(seed=seed)
