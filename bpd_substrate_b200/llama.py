@@ -186,6 +186,8 @@ class DeviceLlama:
 
     def sample(self, seq, tokens, rule, u):
         """Runs the next tokens of `seq`; returns the one that follows them by the rule (sampling.Sampling) and the random number u."""
+        if len(tokens) == 0:
+            raise ValueError("a step needs at least one token")
         if self._sampler is None:
             self._sampler = TokenSampler(self.lib, self.stream)
         pos = np.arange(seq.length, seq.length + len(tokens), dtype=np.int32)

@@ -185,3 +185,12 @@ def test_an_engine_goes_on_after_a_request_that_fails():
 def test_seeds_that_make_no_sense(seed):
     with pytest.raises(ValueError):
         Sampling(seed=seed)
+
+
+def test_a_sampled_step_without_tokens():
+    m = llama.DeviceLlama.__new__(llama.DeviceLlama)
+    m.lib = m.cfg = None                        # (nothing of the device is touched)
+    m._sampler, m.vocab = object(), 96
+    seq = Sequence(0, 1 << 20, 48)
+    with pytest.raises(ValueError):
+        m.sample(seq, [], Sampling(), 0.5)
