@@ -799,3 +799,32 @@ def test_caps_far_from_the_scores(lib, act, kv, cap):
         done(lib, lib.bpd_paged_attention_cuda(desc, d.data_ptr(), 512, o.data_ptr(), 512, c.tokens, 0.5, cap, None, None))
         miss = (o.double().view_as(want) - want).abs() - tolerance(c, want, size, top * (1 + 2.0 ** -20 / (c.D * 2.0 ** -24)), 0.0)
         assert miss.max() <= 0, (new, miss.max().item())
+
+
+@pytest.mark.parametrize("new", [[1] * 4, [1, 90, 1, 20]])
+def test_workspaces_that_are_too_small(lib, new):
+    """A call with less than it needs is refused and leaves its results alone; what the size query says is enough wherever the workspace begins (16-byte aligned)."""
+    c = Cache(8, 2, 128, "bf16", "bf16", 16, [300, 40, 1000, 64], new, 5)
+    c.fill()
+    q = torch.randn(c.tokens, 1024, generator=c.gen).bfloat16().cuda()
+    desc = c.upload()
+    size = lib.bpdq_paged_attention_workspace_bytes(desc, c.tokens, None)
+    ws, o, want = torch.empty(size + 512, dtype=torch.uint8, device="cuda"), torch.full_like(q, 9.0), torch.empty_like(q)
+    base = (ws.data_ptr() + 255) // 256 * 256
+    torch.cuda.synchronize()
+
+    def call(out, at, n):
+        return lib.bpd_paged_attention_ws_cuda(desc, q.data_ptr(), 1024, out.data_ptr(), 1024, c.tokens, 0.1, 0.0, None, at, n, None)
+
+    for at, n in ((base, size - 257), (base + 16, size - 17), (base, 16), (base, 0)):
+        assert call(o, at, n) == -3
+        torch.cuda.synchronize()
+        assert lib.bpdq_last_status() == -3 and (o == 9.0).all()
+        lib.bpdq_clear_status()
+    done(lib, lib.bpd_paged_attention_cuda(desc, q.data_ptr(), 1024, want.data_ptr(), 1024, c.tokens, 0.1, 0.0, None, None))
+    for at, n in ((base, size), (base, size - 256), (base + 16, size), (base + 240, size)):
+        o.fill_(9.0)
+        ws.fill_(255)
+        torch.cuda.synchronize()
+        done(lib, call(o, at, n))
+        assert torch.equal(o, want)
