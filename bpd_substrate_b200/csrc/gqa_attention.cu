@@ -387,15 +387,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// (v0, v1) = hi + lo, 22 bits of mantissa where lo stays above fp16's smallest number (6e-8)
-__device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint32_t& lo)
-{
-    const __half2 h = __floats2half2_rn(v0, v1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(v0 - f.x, v1 - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 
 // One row by one warp, in fp32 and key after key: what a row with values that are not finite falls back to (there the tile's
 // products of masked keys would spread them).

@@ -1,6 +1,8 @@
-// bf16 mma.sync fragments, ldmatrix, cp.async and the two-term bf16 split of fp32 values.
+// bf16 mma.sync fragments, ldmatrix, cp.async and the two-term bf16 and fp16 splits of fp32 values.
 #pragma once
 #include "decoder_device.cuh"
+
+#include <cuda_fp16.h>
 
 namespace bpdq {
 
@@ -33,6 +35,15 @@ __device__ __forceinline__ void split_bf16(float v0, float v1, uint32_t& hi, uin
 {
     hi = pack_bf16(v0, v1);
     lo = pack_bf16(v0 - bf_lo(hi), v1 - bf_hi(hi));
+}
+// (v0, v1) = hi + lo / up, 22 bits of mantissa where lo stays above fp16's smallest number (6e-8)
+__device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint32_t& lo, float up = 1.0f)
+{
+    const __half2 h = __floats2half2_rn(v0, v1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn((v0 - f.x) * up, (v1 - f.y) * up);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // 16 bytes global -> shared; zeros when !valid (the source address is not read then, but must be a valid one).
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid)

@@ -35,25 +35,8 @@ template <> __device__ __forceinline__ void mma_16<__half>(float (&d)[4], const 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename K> __device__ __forceinline__ void split_16(float v0, float v1, uint32_t& hi, uint32_t& lo);
-template <> __device__ __forceinline__ void split_16<bf16>(float v0, float v1, uint32_t& hi, uint32_t& lo) { split_bf16(v0, v1, hi, lo); }
-template <> __device__ __forceinline__ void split_16<__half>(float v0, float v1, uint32_t& hi, uint32_t& lo)
-{
-    const __half2 h = __floats2half2_rn(v0, v1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(v0 - f.x, v1 - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 template <typename K> __device__ __forceinline__ void split_weights(float v0, float v1, uint32_t& hi, uint32_t& lo) { split_bf16(v0, v1, hi, lo); }
-template <> __device__ __forceinline__ void split_weights<__half>(float v0, float v1, uint32_t& hi, uint32_t& lo)
-{
-    const __half2 h = __floats2half2_rn(v0, v1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn((v0 - f.x) * (1.0f / kPsLow<__half>), (v1 - f.y) * (1.0f / kPsLow<__half>));
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
+template <> __device__ __forceinline__ void split_weights<__half>(float v0, float v1, uint32_t& hi, uint32_t& lo) { split_f16(v0, v1, hi, lo, 1.0f / kPsLow<__half>); }
 __device__ __forceinline__ void ldsm4_at(uint32_t (&r)[4], uint32_t p)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
@@ -213,7 +196,7 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 #pragma unroll
                 for (int s = 0; s < kSteps; s++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) split_16<K>(x[s][c].x * down, x[s][c].y * down, qf[m][s][2 * c], qf[m][s][2 * c + 1]);
+                    for (int c = 0; c < 2; c++) split_f16(x[s][c].x * down, x[s][c].y * down, qf[m][s][2 * c], qf[m][s][2 * c + 1]);
             } else {
 #pragma unroll
                 for (int s = 0; s < kSteps; s++)

@@ -64,13 +64,6 @@ template <> __device__ __forceinline__ uint32_t pack_16<__half>(float a, float b
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint32_t& lo)
-{
-    const __half2 h = __floats2half2_rn(v0, v1);
-    const float2 f = __half22float2(h);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = pack_16<__half>(v0 - f.x, v1 - f.y);
-}
 
 // Two fp32 numbers at once.
 __device__ __forceinline__ float2 fma_two(float2 a, float2 b, float2 c)
