@@ -247,7 +247,12 @@ k_paged_split(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     for (int c = 0; c < kSums; c++) out[m][i][c] = 0.0f;
             }
         }
-        if (!mbar_wait_bounded(&bars[warp][stage], (uint32_t)phase, err, 83)) break;
+        if (!mbar_wait_bounded(&bars[warp][stage], (uint32_t)phase, err, 83)) {
+            // no copy is left under way
+#pragma unroll 1
+            for (int v = u; v < src_u; v++) mbar_wait_bounded(&bars[warp][(v - a0) % kStages], (uint32_t)((v - a0) / kStages) & 1u, err, 83);
+            break;
+        }
         const uint32_t kt = ring + stage * 2 * kTile, vt = kt + kTile;
         const int have = min(kPsKeys, it.job.to - it.key);
         const uint32_t gone = missing >> (2 * stage) & 3u, valid = ((1u << have) - 1u) & ~((gone & 1u ? 0xFFu : 0u) | (gone & 2u ? 0xFF00u : 0u));

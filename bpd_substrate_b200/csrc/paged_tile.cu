@@ -103,7 +103,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     constexpr bool f32 = sizeof(A) == 4;
     constexpr int kHalves = Shape::halves, kDepth = Shape::depth;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t q_full, q_empty, k_full[kDepth], k_empty[kDepth], v_full[kDepth], v_empty[kDepth], s_full[2][2], p_full[2][2], o_done[2][2], ml_ready, o1_free, turn[2];
+    __shared__ uint64_t q_full, q_empty, k_full[kDepth], k_empty[kDepth], v_full[kDepth], v_empty[kDepth], s_full[2][2], p_full[2][2], o_done[2][2], ml_ready, o1_free, turn[2], idle[2];
     __shared__ uint64_t item_full[kPtItems], item_empty[kPtItems];
     __shared__ PtItem items[kPtItems];
     __shared__ uint32_t tmem_slot;
@@ -128,6 +128,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         mbar_init(&ml_ready, 4);
         mbar_init(&o1_free, 4);
         mbar_init(&turn[0], 4); mbar_init(&turn[1], 4);
+        mbar_init(&idle[0], 1); mbar_init(&idle[1], 1);
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -465,6 +466,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             if (f32 && !mbar_wait_bounded(&o1_free, (uint32_t)(meets - 1) & 1u, err, 99)) { ok = false; break; }
             taken++;
         }
+        if (!ok) tmem_stored();         // (a role that has given up leaves nothing under way, either: see below)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 || warp == 2) {
@@ -474,7 +476,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
             uint8_t* room = keys ? sk : sv;
             PtItem it = {};
-            int nk = 0, n_items = 0, u = u0;
+            int nk = 0, n_items = 0, asked = 0, u = u0;         // blocks, items; whose queries have been requested
             bool ok = true;
             while (ok) {
                 if (keys) {
@@ -512,7 +514,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         u = it.end;
                     }
                     const int slot = n_items % kPtItems;
-                    if (n_items >= kPtItems && !mbar_wait_bounded(&item_empty[slot], (uint32_t)(n_items / kPtItems - 1) & 1u, err, 101)) break;
+                    if (n_items >= kPtItems && !mbar_wait_bounded(&item_empty[slot], (uint32_t)(n_items / kPtItems - 1) & 1u, err, 101)) { ok = false; break; }
                     if (lane == 0) {
                         items[slot] = it;
                         mbar_arrive(&item_full[slot]);
@@ -520,6 +522,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     __syncwarp();
                     if (it.blocks <= 0) break;
                 } else if (!take(it, n_items, false)) {
+                    ok = it.blocks <= 0;
                     break;
                 }
                 // Queries, once the room of the last item's is free, which is while this one's first keys come.  (The first item's need not wait for any, and the first products wait for them.)
@@ -533,6 +536,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                             for (int h = 0; h < kHalves; h++)
                                 tma_rows_3d(sq + (s * kHalves + h) * kPtPiece, &qmap, 64 * h, it.head * p.share, it.job.first + it.t0 + s * tile_tokens, &q_full);
                     }
+                    asked++;
                     return true;
                 };
                 // a lane per page (box) of a block
@@ -569,6 +573,11 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     nk++;
                 }
                 n_items++;
+            }
+            // Where this role has given up, no copy is left under way when the CTA leaves.  (Else the products have waited for all of them.)
+            if (!ok) {
+                for (int b = max(nk - kDepth, 0); b < nk; b++) mbar_wait_bounded(&full[b % kDepth], (uint32_t)(b / kDepth) & 1u, err, 102);
+                if (asked) mbar_wait_bounded(&q_full, (uint32_t)(asked - 1) & 1u, err, 103);
             }
         } else {
             // ---------------- MMAs.  (What this thread computes between two products is a chain that nothing covers: addresses and descriptors are ready ahead.)
@@ -640,6 +649,11 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         if (t + 2 < steps) ok = scores(t + 2);
                     }
                     taken++;
+                }
+                // nor a product, when tensor memory is given back
+                if (it.blocks > 0) {
+                    umma_commit(&idle[s]);
+                    mbar_wait_bounded(&idle[s], 0, err, 104);
                 }
             }
         __syncwarp();
