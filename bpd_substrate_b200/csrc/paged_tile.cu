@@ -544,7 +544,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 const int* table = p.table + (size_t)it.job.seq * p.max_pages;
                 auto entry_of = [&](int b) {
                     const int key = it.from + b * kPtKeys + lane * box_rows;
-                    return lane < boxes && key < it.job.to ? table[key >> p.log_page] : -2;
+                    return lane < boxes && key < it.job.to ? max(table[key >> p.log_page], -1) : -2;        // (-2: none is needed)
                 };
                 int entry = entry_of(0);
                 for (int b = 0; b <= it.blocks; b++) {

@@ -828,3 +828,31 @@ def test_workspaces_that_are_too_small(lib, new):
         torch.cuda.synchronize()
         done(lib, call(o, at, n))
         assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("entry", [-1, -2, -3, -2 ** 31, 2 ** 31 - 1])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_every_bad_page_is_reported(lib, act, kv, new, entry):
+    """Whatever number stands in its place, to appending and to attention over few rows and many."""
+    c = Cache(4, 2, 64, act, kv, 16, [100, 30], [new, new], 3, ragged=True)
+    c.fill()
+    c.table[0, 3] = entry
+    q = torch.randn(c.tokens, 256, generator=c.gen).to(TYPES[act][0])
+    want, size, top = attention_oracle(c, q, 0.1, 0.0)
+    desc, d = c.upload(), q.cuda()
+    o = torch.full_like(d, 9.0)
+    torch.cuda.synchronize()
+    assert lib.bpd_paged_attention_cuda(desc, d.data_ptr(), 256, o.data_ptr(), 256, c.tokens, 0.1, 0.0, None, None) == 0
+    torch.cuda.synchronize()
+    status = lib.bpdq_last_status()
+    lib.bpdq_clear_status()
+    assert status == -4
+    assert ((o.double().view_as(want) - want).abs() <= tolerance(c, want, size, top, 0.0)).all()
+    c.d_len[0] = 48                                          # the new tokens' first page is the bad one
+    torch.cuda.synchronize()
+    assert lib.bpd_paged_append_cuda(desc, None, 0, None, 0, d.data_ptr(), 256, d.data_ptr() + 128 * d.element_size(), 256, c.tokens, 0, 0, None, None) == 0
+    torch.cuda.synchronize()
+    status = lib.bpdq_last_status()
+    lib.bpdq_clear_status()
+    assert status == -4
