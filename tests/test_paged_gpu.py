@@ -856,3 +856,10 @@ def test_every_bad_page_is_reported(lib, act, kv, new, entry):
     status = lib.bpdq_last_status()
     lib.bpdq_clear_status()
     assert status == -4
+
+
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("new", [[1], [5], [70], [1, 300, 1]])
+def test_a_long_context(lib, act, kv, new):
+    """130 000 positions, for one token, a few, a portion, and a portion of a prompt beside it."""
+    attention_case(lib, 8, 2, 128, act, kv, 32, [130000, 10, 900][:len(new)], new, seed=len(new), ragged=True)
