@@ -81,6 +81,13 @@ __device__ __forceinline__ float2 add_two(float2 a, float2 b)
     return d;
 }
 
+// All products of this thread so far.  (Out of line: in its place in the role that issues them, where it is hardly ever needed, a capped prompt of 2000 took 120.4 us for 117.9.)
+__device__ __noinline__ void products_end(uint64_t* bar, int* err)
+{
+    umma_commit(bar);
+    mbar_wait_bounded(bar, 0, err, 104);
+}
+
 // An item: a key head's rows of some tokens of a job.
 struct PtItem {
     PagedJob job;
@@ -650,11 +657,8 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     }
                     taken++;
                 }
-                // nor a product, when tensor memory is given back
-                if (it.blocks > 0) {
-                    umma_commit(&idle[s]);
-                    mbar_wait_bounded(&idle[s], 0, err, 104);
-                }
+                // nor a product, when tensor memory is given back.  (Where no item has come within the limit the last one's products ended long ago.)
+                if (!ok) products_end(&idle[s], err);
             }
         __syncwarp();
         }
