@@ -549,10 +549,9 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 // a lane per page (box) of a block
                 const int box_rows = p.page < kPtKeys ? p.page : kPtKeys, boxes = kPtKeys / box_rows;
                 const int* table = p.table + (size_t)it.job.seq * p.max_pages;
-                auto entry_of = [&](int b) {
-                    const int key = it.from + b * kPtKeys + lane * box_rows;
-                    return lane < boxes && key < it.job.to ? max(table[key >> p.log_page], -1) : -2;        // (-2: none is needed)
-                };
+                auto needed = [&](int b) { return lane < boxes && it.from + b * kPtKeys + lane * box_rows < it.job.to; };
+                // (on its way while the block before is requested: nothing is made of it here)
+                auto entry_of = [&](int b) { return needed(b) ? table[(it.from + b * kPtKeys + lane * box_rows) >> p.log_page] : -1; };
                 int entry = entry_of(0);
                 for (int b = 0; b <= it.blocks; b++) {
                     if (!f32 && keys && b == (n_items ? min(kDepth, it.blocks) : 0) && !(ok = queries())) break;
@@ -560,7 +559,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     const int slot = nk % kDepth, now = entry;
                     if (b + 1 < it.blocks) entry = entry_of(b + 1);
                     const bool have = now >= 0 && now < p.n_pages;
-                    if (now != -2 && !have) report(err, 82);
+                    if (!have && needed(b)) report(err, 82);
                     const unsigned who = __ballot_sync(0xFFFFFFFFu, have);
                     if (nk >= kDepth && !mbar_wait_bounded(&empty[slot], (uint32_t)(nk / kDepth - 1) & 1u, err, 85 + !keys)) { ok = false; break; }
                     if (lane == 0) {
