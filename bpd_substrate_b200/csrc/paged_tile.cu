@@ -81,13 +81,6 @@ __device__ __forceinline__ float2 add_two(float2 a, float2 b)
     return d;
 }
 
-// All products of this thread so far.  (Out of line: in its place in the role that issues them, where it is hardly ever needed, a capped prompt of 2000 took 120.4 us for 117.9.)
-__device__ __noinline__ void products_end(uint64_t* bar, int* err)
-{
-    umma_commit(bar);
-    mbar_wait_bounded(bar, 0, err, 104);
-}
-
 // An item: a key head's rows of some tokens of a job.
 struct PtItem {
     PagedJob job;
@@ -114,6 +107,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     __shared__ uint64_t item_full[kPtItems], item_empty[kPtItems];
     __shared__ PtItem items[kPtItems];
     __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up;                             // a role has
     __shared__ unsigned short s_missing[8];             // of a block: groups of eight keys without a page; softmax is two blocks behind the copies' kDepth at most
     __shared__ float2 s_ml[kPtRows];
     __shared__ uint8_t* s_row[2][kPtRows];              // where rows go; null: nowhere
@@ -127,6 +121,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         if (!f32) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
     }
     if (tid == 0) {
+        gave_up = 0;
         mbar_init(&q_full, f32 ? kPtWarps : 1);
         mbar_init(&q_empty, kPtWarps);
         for (int i = 0; i < kDepth; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 2); }
@@ -473,7 +468,10 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             if (f32 && !mbar_wait_bounded(&o1_free, (uint32_t)(meets - 1) & 1u, err, 99)) { ok = false; break; }
             taken++;
         }
-        if (!ok) tmem_stored();         // (a role that has given up leaves nothing under way, either: see below)
+        if (!ok) {
+            tmem_stored();
+            gave_up = 1;
+        }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 || warp == 2) {
@@ -582,6 +580,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             }
             // Where this role has given up, no copy is left under way when the CTA leaves.  (Else the products have waited for all of them.)
             if (!ok) {
+                gave_up = 1;
                 for (int b = max(nk - kDepth, 0); b < nk; b++) mbar_wait_bounded(&full[b % kDepth], (uint32_t)(b / kDepth) & 1u, err, 102);
                 if (asked) mbar_wait_bounded(&q_full, (uint32_t)(asked - 1) & 1u, err, 103);
             }
@@ -656,8 +655,7 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     }
                     taken++;
                 }
-                // nor a product, when tensor memory is given back.  (Where no item has come within the limit the last one's products ended long ago.)
-                if (!ok) products_end(&idle[s], err);
+                if (!ok) gave_up = 1;
             }
         __syncwarp();
         }
@@ -665,6 +663,13 @@ k_paged_tile(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     if (p.mark && warp < 4) mark_tokens(p, tid, 128, err);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (gave_up) {                      // no product is left under way, either, when tensor memory is given back: the threads that have issued them wait
+        if ((warp == 1 || warp == 3) && elect_one()) {
+            umma_commit(&idle[warp >> 1]);
+            mbar_wait_bounded(&idle[warp >> 1], 0, err, 104);
+        }
+        __syncthreads();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
