@@ -3,8 +3,8 @@
 //
 // Pair (x, y) with frequency f at position p becomes (x cos a - y sin a, x sin a + y cos a), a = p f.  The angle is formed and reduced to half
 // turns in 64 bits: fp32 would lose 2^-24 p f of it.
-// Bound by memory where there are many tokens, by the launch where there are few: 7683 tokens of 32 heads on 8 of 128 in bf16 (189 MB) 42 us, 4.5 TB/s, for which
-// a copy of as many bytes takes 65; 16 tokens of fp32 2.6 us.  (Four tokens per CTA, the next loads ahead of the stores: 43; two: 46; 16-byte units: 41 to 54.)
+// Bound by the launch where there are few tokens: 16 of fp32 2.6 us.  Many: 7683 of 32 heads on 8 of 128 in bf16 (189 MB) 42 us, 4.5 TB/s, 70 % of the measured copy rate: a
+// CTA's loads wait for its token's sequence, the page's number and the angles, three steps that follow one another.  (Four tokens per CTA, the next loads ahead of the stores: 43; two: 46; 16-byte units: 41 to 54.)
 #include "paged.cuh"
 
 namespace bpdq {

@@ -28,7 +28,7 @@ struct PagedArgs {
     int4* own;                  // [tokens][heads]: what k_paged_join finds of a row's own positions
     int4* prefix;               // the same of its group's
     float *own_o, *prefix_o;    // [tokens * heads][dim_pad]: parts that are whole, unnormalised
-    float2 *own_ml, *prefix_ml; // their maxima (in units of log2) and sums
+    float2 *own_ml, *prefix_ml; // what their sums count from (maxima, in units of log2, less the kernel's shift) and sums of weights
     float *split_o, *tile_o;    // parts of items that several CTAs share: [2 * CTA + which][rows][dim_pad]
     float2 *split_ml, *tile_ml;
     float* tile_sums;           // k_paged_tile of fp32: what a stream has put aside, [2 * CTA + stream][dim_pad / 4][rows of a stream][4]
@@ -74,7 +74,7 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
 
 // cap tanh(x / cap): of fp32 results by CUDA's function, of rounded ones by 1 - 2 / (1 + e^(2 x / cap)), off by 2^-22 of the cap.  That shows in the weights where the cap is far
 // above the scores, and the approximate divisions have an end of their own: of such caps scores are off by 2^-20 of themselves, below 0.3 caps by the first five terms of tanh's series
-// (the sixth: 2^-24).  (A bf16 prompt of 2000, 32 heads on 8 of 128: cap 30 113 us, 200 141.)
+// (the sixth: 2^-24).  (A bf16 prompt of 2000, 32 heads on 8 of 128: cap 30 117 us, 200 145.)
 enum CapKind { kCapNone = 0, kCapNear = 1, kCapFar = 2 };
 static inline CapKind cap_kind(float cap, bool f32) { return cap > 0.0f ? (f32 || (cap >= 1.0f / 1048576.0f && cap <= 64.0f) ? kCapNear : kCapFar) : kCapNone; }
 template <bool f32, int kCap> __device__ __forceinline__ float capped(float x, float cap)

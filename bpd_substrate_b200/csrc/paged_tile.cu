@@ -14,7 +14,8 @@
 // O stays in tensor memory and is rescaled only when a row's maximum has grown by much since the last time.  Weights are rounded to the cache's type: half
 // a step (2^-9 of a bf16 weight on average) of each, which the sum over keys averages to below the result's own rounding.  fp32 activations bring queries and weights as two
 // fp16 numbers each: four products where 16 bits take two, and one tile per item.
-// One prompt of 8000 tokens, 32 heads on 8 of 128 in bf16: 522 us, 1005 TFLOP/s of a measured 1688; three portions of 2000 after up to 2000: 133 us with the join (14).  Bound by what
+// One prompt of 8000 tokens, 32 heads on 8 of 128 in bf16: 526 us with the launches behind it, 997 TFLOP/s of a measured 1688; three portions of 2000 after up to 2000: 136 us, 14 of it
+// the join and 4 the kernel for few rows, which has nothing to do.  Bound by what
 // the streams and the tensor pipe hand to each other: some 2400 cycles for a step of both streams, 1024 of them products.  64 tokens on a prefix of 16000 (8 items on 148
 // CTAs): 40 us, half of it until the first scores.
 #include "paged_attention.cuh"

@@ -54,8 +54,8 @@ int bpdq_sm_count(void);
  * Some entries need device scratch beyond their inputs and outputs (quantized activations, states and
  * partial sums, the forward pass's vectors): the many-token products bpd_qmm_q4k_q8k_cuda (from 2 tokens
  * on) / _mma_cuda / _tc5_cuda / gpu_matmul_q4k, bpd_qmatmul_q8_0_tiles_cuda and bpd_qmatmul_q8_0_llamafile_cuda,
- * bpd_llama_forward*_cuda, and of the decoders' single mechanisms bpd_decayed_scan_cuda (long bf16 portions),
- * bpd_latent_attention_cuda and bpd_delta_rule_cuda.  The products and the forward have two forms, the
+ * bpd_llama_forward*_cuda, bpd_paged_attention_cuda, and of the decoders' single mechanisms bpd_decayed_scan_cuda (long bf16 portions),
+ * bpd_latent_attention_cuda and bpd_delta_rule_cuda.  The products, the forward and the attention over pages have two forms, the
  * mechanisms the second alone:
  *   *_ws_cuda(..., workspace, workspace_bytes, stream): the caller owns the scratch (16-byte aligned, at
  *     least the matching *_workspace_bytes()).  Nothing is allocated and no state is shared between calls:
@@ -632,7 +632,8 @@ typedef struct {
  * groups NULL: none.  A sequence's sums are split over the GPU by a rule on all lengths of the call: its last bits may depend
  * on what else is in the batch.  Up to 128 query heads per key head, 1280 sequences and
  * groups together; batch * kv_heads * max_pages * page up to 2^33 and,
- * in whole numbers, (2 n_tokens / (128 / (heads / kv_heads)) + 2 batch) * kv_heads * (max_pages * page / 128 + 3) below 2^31.  Scratch: see "scratch memory" above; its size does not depend on lengths. */
+ * in whole numbers, (2 n_tokens / (128 / (heads / kv_heads)) + 2 batch) * kv_heads * (max_pages * page / 128 + 3) below 2^31.  Scratch: see "scratch memory" above; its size does not depend on lengths, and with groups grows
+ * by two rows of fp32 numbers per token and query head of the call, whether in a group or not (8000 tokens of 32 heads of 128: 262 MB). */
 int bpd_paged_attention_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q, void* o, int ld_o, int n_tokens, float scale, float cap,
                              const bpdq_paged_groups* groups, void* stream);
 size_t bpdq_paged_attention_workspace_bytes(const bpdq_paged_kv* kv, int n_tokens, const bpdq_paged_groups* groups);
@@ -641,9 +642,9 @@ int bpd_paged_attention_ws_cuda(const bpdq_paged_kv* kv, const void* q, int ld_q
 /* A token per row of logits [rows][ld] (ld >= vocab, vocab up to 262144) from given random numbers u[r] in [0, 1).  With weights w_i = exp((x_i - max) / temperature), sorted by x (the lowest
  * index first among equals): the first top_k of them (0 or less: all), of these the fewest whose weights reach top_p of theirs (1 or more: all; one at least), of these
  * the ones with w >= min_p (0: all); then the first index, in the vocabulary's order, at which the sum of the kept weights exceeds u times
- * their total.  temperature 0 (or anything not above 0): the largest logit.  Settings are device arrays [rows]; NULL: temperature 1, no cut.  NaN and -inf logits
+ * their total.  temperature 0 (or anything not above 0): the largest logit; above 8e36: as 8e36.  Settings are device arrays [rows]; NULL: temperature 1, no cut.  NaN and -inf logits
  * are never chosen; +inf beats all others; a row that has nothing else gives token -1 and log probability -inf.  logprob (or NULL): ln(w / total) of the token among the
- * kept.  Weights are held to 2^-45 of the largest (a token with less is never chosen) and added as whole numbers, so a token depends neither on the order of sums nor on
+ * kept.  -0 and 0 are equal.  Weights are held to 2^-45 of the largest (a token with less is never chosen) and added as whole numbers, so a token depends neither on the order of sums nor on
  * what else is in the batch. */
 int bpd_sample_cuda(const void* logits, int logits_type, int ld, int rows, int vocab, const float* temperature, const int32_t* top_k, const float* top_p,
                     const float* min_p, const float* u, long long* token, float* logprob, void* stream);
