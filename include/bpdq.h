@@ -625,7 +625,7 @@ typedef struct {
 /* o[t][h] = sum_j softmax_j(s_j) v_j over the positions up to the token's own, s = scale q.k, with cap > 0 then cap tanh(s / cap).  The tokens' own keys and values are in the cache
  * already (bpd_paged_append_cuda); q and o rows are ld_* elements apart, o may be q, with the same ld.  What lies in a page's other places is never looked at; the values
  * at a sequence's positions, the call's new ones too, have to be finite (those behind a token meet weights of 0). 
- * How exact: scores are off by up to (dim + 16) 2^-24 |scale| sum_i |q_i k_i|, and a weight by as much of itself.  With fp32 activations queries and weights enter the tensor cores as two
+ * How exact: scores are off by up to (dim + 16) 2^-24 |scale| sum_i |q_i k_i| (with fp32 activations also 2^-25 |scale| max_i |q_i| sum_i |k_i|), and a weight by as much of itself.  With fp32 activations queries and weights enter the tensor cores as two
  * fp16 numbers each, and sums of more than 256 keys are added as fp32 numbers: beyond what scores are off by, results are within 5e-6 of sum_j w_j |v_j| and, since fp16 has an end, 2^-36 of
  * w_max sum_j |v_j|.  With 16-bit types weights may be rounded to the cache's type (where a sequence or a group has more than 8 rows): half a step of it of sum_j w_j |v_j|, of fp16
  * also 2^-32 of w_max sum_j |v_j|, and the result's rounding.
